@@ -553,6 +553,24 @@ int rte_router_aux_fwd(const float* probs, const float* edepth, const float* ema
 int rte_router_aux_bwd(const float* mean_prob, const float* g_load, const float* g_depth, int B, int R,
                        float lambda_load, float lambda_depth, float* dprobs, float* dedepth, void* stream);
 
+/* ---- load balance of routed pools (no counterpart in the reference, whose router_aux_losses weigh
+ *      recipes) ----
+ * logits [T, C] (f32, or bf16 when f32 == 0; row stride ld), ids int32 [T, k] = the pools of each
+ * row (outside [0, C): none; a pool named twice counts twice), mask (bool bytes [T], NULL: all) =
+ * rows that take part; rows whose logits are all -inf take none either.  With n such rows, p =
+ * softmax of a row, counts[c] = pairs sent to c, f_c = counts[c] / sum counts:
+ *   out[0] = C sum_c f_c mean_t p_tc     out[1] = mean_t lse_t^2     (0 when n == 0)
+ * frac f32 [C + 1] = f and 1 / n, for the backward:
+ *   dlogits = p (g_balance C (f - sum f p) + 2 g_z lse) / n, in the logits' type, dense [T, C]; rows
+ *   without part get 0.  g_balance, g_z: device scalars, NULL = 0.
+ * C <= 1024.  Two launches; sums in a fixed order. */
+size_t rte_pool_balance_workspace_bytes(int T, int C);
+int rte_pool_balance_fwd(const void* logits, int64_t ld, int f32, int T, int C, const int32_t* ids, int k,
+                         const uint8_t* mask, float* out, int32_t* counts, float* frac, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int rte_pool_balance_bwd(const void* logits, int64_t ld, int f32, int T, int C, const uint8_t* mask,
+                         const float* frac, const float* g_balance, const float* g_z, void* dlogits, void* stream);
+
 /* ---- audit sampler and usage statistics (replaces AuditEngine.compute_audit_prob and the
  *      fixed-count branch of sample_mask_with_prob, rte/audit.py:79-132, and the bincount EMAs of
  *      RecipeBank.update_usage / the audit coverage update) ----
@@ -600,6 +618,46 @@ size_t rte_adamw_workspace_bytes(int n_tensors, int n_blocks, int n_groups);
 int rte_adamw_step(const void* rows, int n_tensors, const int32_t* blocks, const int32_t* first_block, int n_blocks,
                    const double* hyper, int n_groups, const int32_t* metric_lr_group, int n_metrics, float clip_max,
                    const float* found_inf, float* metrics, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- log probabilities of given tokens, entropies and top alternatives (no counterpart in the
+ *      reference; beside rte_ce_fwd) ----
+ * logits [T, V] (f32, or bf16 when f32 == 0; row stride ld in elements, any alignment of the element
+ * type), tokens int64 [T].  p = softmax(logits / temperature) per row:
+ *   logprob[t] = log p[tokens[t]]  (0 for a negative token, NaN for one past the vocabulary)
+ *   entropy[t] = -sum p log p
+ *   top_ids int32 / top_logprobs f32 [T, n_top]: the largest logits and their log p, value descending,
+ *   ties to the lower column, NaN first.  n_top <= min(128, V).
+ * A row with no logit above -inf has logprob and top_logprobs -inf and entropy 0; a NaN or +inf logit
+ * makes the row's results NaN.  stats f32 [T, 2] (NULL without a backward): row maximum, log sum.
+ * bwd: dlogits [T, V] dense in the logits' type = (g_logprob ([v = token] - p) - g_entropy p (log p +
+ * entropy)) / temperature; g_logprob / g_entropy f32 [T], NULL = 0; padded tokens give no gradient
+ * through logprob, rows with no logit above -inf none at all. */
+size_t rte_token_logprobs_workspace_bytes(int T, int V, int n_top);
+int rte_token_logprobs_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int64_t* tokens,
+                           float temperature, int n_top, float* logprob, float* entropy, float* top_logprobs,
+                           int32_t* top_ids, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V, const int64_t* tokens,
+                           float temperature, const float* stats, const float* entropy, const float* g_logprob,
+                           const float* g_entropy, void* dlogits, void* stream);
+
+/* ---- divergence from a teacher's top logits (no counterpart in the reference, whose
+ *      macro_distill_loss needs the teacher's whole row) ----
+ * logits as above; ids int32 [T, K] = columns of the teacher's list (negative: no entry; the first
+ * entry of a column counts), teacher f32 [T, K].  q = softmax(logits / temperature):
+ *   tail 0: p = softmax over the list of teacher / temperature,
+ *           loss = temperature^2 sum_j p_j (log p_j - log q_j)
+ *   tail 1: teacher = log probabilities at that temperature, p_j = e^teacher_j, r = max(1 - sum p_j, 0),
+ *           loss = temperature^2 (sum_j p_j (log p_j - log q_j) + r (log r - log q(not listed)))
+ * A row without entries (tail 0: or without a finite one) has loss 0 and no gradient; an id past the
+ * vocabulary makes the loss NaN and the gradient 0.  K <= 128.  stats f32 [T, 6], NULL without a backward.
+ * bwd: dlogits [T, V] dense in the logits' type, for g f32 [T]. */
+size_t rte_topk_distill_workspace_bytes(int T, int V, int K);
+int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
+                         const float* teacher, int K, float temperature, int tail, float* loss, float* stats,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int rte_topk_distill_bwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
+                         const float* teacher, int K, float temperature, int tail, const float* stats,
+                         const float* g, void* dlogits, void* stream);
 
 /* ---- hot-vs-exact distillation losses + alignment metrics of the audit (replaces
  *      macro_distill_loss rte/macro.py:394-471 and macro_alignment_metrics :499-546 on the

@@ -131,6 +131,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rte_router_mlp_bwd": (_I, [_P] * 6 + [_I, _I, _I, _I, _P, _I, _F] + [_P] * 9 + [_P]),
     "rte_router_aux_fwd": (_I, [_P, _P, _P, _I, _I, _F, _F, _F, _F, _P, _P, _P]),
     "rte_router_aux_bwd": (_I, [_P, _P, _P, _I, _I, _F, _F, _P, _P, _P]),
+    "rte_pool_balance_workspace_bytes": (_SZ, [_I, _I]),
+    "rte_pool_balance_fwd": (_I, [_P, _I64, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _SZ, _P]),
+    "rte_pool_balance_bwd": (_I, [_P, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
     "rte_audit_sample_fixed": (_I, [_P, _P, _P, _P, _I, _I, _I] + [_F] * 8 + [_P, _P, _P, _P, _P]),
     "rte_count_ema": (_I, [_P, _P, _I, _P, _I, _F, _P]),
     "rte_nonfinite": (_I, [_P, _P, _P, _P]),
@@ -166,6 +169,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rte_distill_workspace_bytes": (_SZ, [_I, _I]),
     "rte_distill_fwd": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _I, _F, _F, _P, _P, _P, _P, _SZ, _P]),
     "rte_distill_bwd": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _I, _F, _F, _P, _P, _P, _SZ, _P, _P, _P]),
+    "rte_token_logprobs_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "rte_token_logprobs_fwd": (_I, [_P, _I64, _I, _I, _I, _P, _F, _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "rte_token_logprobs_bwd": (_I, [_P, _I64, _I, _I, _I, _P, _F, _P, _P, _P, _P, _P, _P]),
+    "rte_topk_distill_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "rte_topk_distill_fwd": (_I, [_P, _I64, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _P, _SZ, _P]),
+    "rte_topk_distill_bwd": (_I, [_P, _I64, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _P, _P]),
     "rte_audit_correct_fwd": (_I, [_P, _P, _I, _I, _P, _I, _P, _F, _I, _P, _P, _P, _P, _P]),
     "rte_audit_correct_bwd": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _P]),
     "rte_cast_f32_bf16": (_I, [_P, _I64, _P, _P]),

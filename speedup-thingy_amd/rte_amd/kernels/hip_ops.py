@@ -15,10 +15,11 @@ from __future__ import annotations
 import ctypes
 import math
 import threading
-from contextlib import contextmanager
+from contextlib import contextmanager, nullcontext
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from rte_amd import _lib
 from rte_amd._lib import call, ptr
@@ -1458,6 +1459,70 @@ def router_aux(probs, expected_depth, usage_ema, *, coverage_min: float, lambda_
     return {"load": load, "cover": cover, "depth": depth}
 
 
+class PoolBalanceFn(torch.autograd.Function):
+    """Balance loss, router z-loss and counts of routed pools (rte_pool_balance_*)."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, mask):
+        dev = logits.device
+        C, k = logits.shape[-1], ids.shape[-1]
+        lg, ld = _logit_rows(logits)
+        T = lg.shape[0]
+        ic = _ids32(ids.reshape(T, k))
+        mc = None if mask is None else mask.reshape(T).contiguous().view(torch.uint8)
+        out = torch.empty((2,), dtype=F32, device=dev)
+        counts = torch.empty((C,), dtype=torch.int32, device=dev)
+        frac = torch.empty((C + 1,), dtype=F32, device=dev)
+        with _on_device(dev):
+            ws = _scratch(_lib.load().rte_pool_balance_workspace_bytes(T, C), dev)
+            call("rte_pool_balance_fwd", ptr(lg), ld, int(lg.dtype == F32), T, C, ptr(ic), k, ptr(mc), ptr(out),
+                 ptr(counts), ptr(frac), ptr(ws), ws.numel(), _s())
+        ctx.save_for_backward(lg, mc, frac)
+        ctx.meta = (logits.shape, T, C, ld)
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return out[0], out[1], counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_bal, g_z, _g_counts):
+        if g_bal is None and g_z is None:
+            return None, None, None
+        lg, mc, frac = ctx.saved_tensors
+        shape, T, C, ld = ctx.meta
+        gb = None if g_bal is None else g_bal.reshape(1).contiguous().to(F32)
+        gz = None if g_z is None else g_z.reshape(1).contiguous().to(F32)
+        dx = torch.empty((T, C), dtype=lg.dtype, device=lg.device)
+        with _on_device(lg.device):
+            call("rte_pool_balance_bwd", ptr(lg), ld, int(lg.dtype == F32), T, C, ptr(mc), ptr(frac), ptr(gb), ptr(gz),
+                 ptr(dx), _s())
+        return dx.view(shape), None, None
+
+
+def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(balance, z, counts int32 [C]) of router logits [..., C] (float32 or bfloat16, C <= 1024) whose rows
+    were sent to the pools ids [..., k] (route_topk's; outside [0, C): none).
+
+    balance = C sum_c f_c mean_t softmax(logits)_tc with f_c the share of the pairs that pool c got (1 when
+    both are even), z = mean_t logsumexp(logits_t)^2.  mask (bool [...]) leaves rows out, padding for one,
+    whatever their logits hold; rows whose logits are all -inf take no part either.  Both losses are
+    differentiable in the logits; the counts are exact and carry no gradient."""
+    _lib.require_device_tensors("pool_balance", logits, ids, mask)
+    _same_device("pool_balance", logits, ids, mask)
+    _io_flag(logits, "pool_balance")
+    lead = logits.shape[:-1]
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] <= 1024:
+        raise ValueError(f"pool_balance: need [..., C] logits with 1 <= C <= 1024, got {tuple(logits.shape)}")
+    if ids.ndim < 1 or ids.shape[:-1] != lead or ids.shape[-1] < 1:
+        raise ValueError(f"pool_balance: ids {tuple(ids.shape)} do not match logits {tuple(logits.shape)}")
+    _whole_numbers("pool_balance", ids)
+    if ids.numel() >= 1 << 31:
+        raise ValueError("pool_balance: fewer than 2^31 (row, pool) pairs expected")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != lead):
+        raise ValueError(f"pool_balance: mask must be bool {tuple(lead)}, got {mask.dtype} {tuple(mask.shape)}")
+    return PoolBalanceFn.apply(logits, ids, mask)
+
+
 # ----------------------------------------------------------------------------- LM head + cross-entropy
 
 class LMHeadCEFn(torch.autograd.Function):
@@ -1534,6 +1599,268 @@ def select_logit_rows(logits: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     sink = _RowSink(idx)
     node.row_sinks = getattr(node, "row_sinks", []) + [sink]
     return SelectRowsFn.apply(logits, idx, sink)
+
+
+# ----------------------------------------------------------------------------- log probabilities of tokens
+
+MAX_TOP = 128  # alternatives per row, of token_logprobs and topk_distill
+
+
+def _logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x [..., V] as [T, V] rows with contiguous columns (a view where its strides allow) and their stride."""
+    V = x.shape[-1]
+    x2 = x.detach().reshape(-1, V)
+    if x2.stride(1) != 1 and V > 1:
+        x2 = x2.contiguous()
+    return x2, x2.stride(0)
+
+
+def _same_device(op: str, *tensors) -> None:
+    ts = [t for t in tensors if t is not None]
+    if any(t.device != ts[0].device for t in ts):
+        raise RuntimeError(f"{op}: operands are on different devices ({', '.join(str(t.device) for t in ts)})")
+
+
+def _on_device(dev: torch.device):
+    """Makes dev the current device for a launch, where it is another one."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
+    """A call's own workspace (the allocator keeps those of a captured call with its graph)."""
+    return torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+
+
+def _whole_numbers(op: str, t: torch.Tensor) -> None:
+    if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise TypeError(f"{op}: whole numbers expected, got {t.dtype}")
+
+
+def _ids32(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous in 32 bits; wider numbers that do not fit stay out of every range."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, 0x7FFFFFFF)
+    return t.contiguous().to(torch.int32)
+
+
+def _temperature(op: str, t: float) -> float:
+    t = float(t)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{op}: temperature must be in [1e-6, 1e6], got {t}")
+    return t
+
+
+def _check_logits(op: str, logits: torch.Tensor) -> None:
+    _io_flag(logits, op)
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] < 1 << 30 or logits.numel() // logits.shape[-1] >= 1 << 31:
+        raise ValueError(f"{op}: unsupported logits {tuple(logits.shape)}")
+
+
+def _row_grad(g, T: int):
+    return None if g is None else g.reshape(T).contiguous().to(F32)
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    """Per row of logits: the token's log probability, the entropy and the top alternatives
+    (rte_token_logprobs_*); the backward is one pass from the saved row statistics."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, n_top: int, temperature: float):
+        dev = logits.device
+        lead, V = logits.shape[:-1], logits.shape[-1]
+        lg, ld = _logit_rows(logits)
+        T = lg.shape[0]
+        tk = tokens.reshape(T).contiguous().to(torch.int64)
+        lp = torch.empty((T,), dtype=F32, device=dev)
+        ent = torch.empty((T,), dtype=F32, device=dev)
+        top_lp = torch.empty((T, n_top), dtype=F32, device=dev)
+        top_ids = torch.empty((T, n_top), dtype=torch.int32, device=dev)
+        need = ctx.needs_input_grad[0]
+        stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
+        with _on_device(dev):
+            ws = _scratch(_lib.load().rte_token_logprobs_workspace_bytes(T, V, n_top), dev)
+            call("rte_token_logprobs_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, n_top,
+                 ptr(lp), ptr(ent), ptr(top_lp), ptr(top_ids), ptr(stats), ptr(ws), ws.numel(), _s())
+        if need:
+            ctx.save_for_backward(lg, tk, stats, ent)
+            ctx.meta = (logits.shape, ld, temperature)
+        ctx.mark_non_differentiable(top_lp, top_ids)
+        ctx.set_materialize_grads(False)
+        return lp.view(lead), ent.view(lead), top_lp.view(*lead, n_top), top_ids.view(*lead, n_top)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, _g_top, _g_ids):
+        if g_lp is None and g_ent is None:
+            return None, None, None, None
+        lg, tk, stats, ent = ctx.saved_tensors
+        shape, ld, temperature = ctx.meta
+        T, V = lg.shape
+        gl, ge = _row_grad(g_lp, T), _row_grad(g_ent, T)
+        dx = torch.empty((T, V), dtype=lg.dtype, device=lg.device)
+        with _on_device(lg.device):
+            call("rte_token_logprobs_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, ptr(stats),
+                 ptr(ent), ptr(gl), ptr(ge), ptr(dx), _s())
+        return dx.view(shape), None, None, None
+
+
+def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
+    """(logprob, entropy, top_logprobs, top_ids) of softmax(logits / temperature), logits [..., V] in float32 or
+    bfloat16 (rows may be strided), tokens [...] whole numbers.
+
+    logprob [...] float32: log p of the token; a negative token (padding, -100) gives 0 and no gradient, one past
+    the vocabulary NaN.  entropy [...] float32: -sum p log p.  top_logprobs float32 / top_ids int32 [..., n_top]:
+    the n_top <= 128 largest logits, value descending, ties to the lower id, NaN first.  logprob and entropy are
+    differentiable; the alternatives carry no gradient (they make topk_distill's targets).  A row with no logit
+    above -inf has log probabilities -inf, entropy 0 and gradient 0; a NaN or +inf logit makes its row NaN."""
+    _lib.require_device_tensors("token_logprobs", logits, tokens)
+    _same_device("token_logprobs", logits, tokens)
+    _check_logits("token_logprobs", logits)
+    _whole_numbers("token_logprobs", tokens)
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+    if not 0 <= int(n_top) <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: n_top must be in [0, min({MAX_TOP}, V)], got {n_top}")
+    return TokenLogprobsFn.apply(logits, tokens, int(n_top), _temperature("token_logprobs", temperature))
+
+
+class LMHeadLogprobsFn(torch.autograd.Function):
+    """token_logprobs' first two results of hidden @ W^T without keeping the logits: the backward computes
+    them again, a range of tokens at a time."""
+
+    ROWS = 2048
+
+    @staticmethod
+    def forward(ctx, hidden, w, tokens, temperature: float):
+        shape = hidden.shape
+        hb = hidden.reshape(-1, shape[-1]).contiguous().to(BF16)
+        wb = cast_bf16(w)
+        T, V = hb.shape[0], wb.shape[0]
+        dev = hb.device
+        tk = tokens.reshape(T).contiguous().to(torch.int64)
+        lp = torch.empty((T,), dtype=F32, device=dev)
+        ent = torch.empty((T,), dtype=F32, device=dev)
+        stats = torch.empty((T, 2), dtype=F32, device=dev)
+        with _on_device(dev):
+            for lo in range(0, T, LMHeadLogprobsFn.ROWS):
+                hi = min(T, lo + LMHeadLogprobsFn.ROWS)
+                logits = gemm(hb[lo:hi], wb, out_f32=True)
+                call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0, ptr(lp[lo:]),
+                     ptr(ent[lo:]), None, None, ptr(stats[lo:]), None, 0, _s())
+        ctx.save_for_backward(hb, wb, tk, stats, ent)
+        ctx.meta = (shape, hidden.dtype, w.dtype, temperature)
+        ctx.set_materialize_grads(False)
+        return lp.view(shape[:-1]), ent.view(shape[:-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent):
+        if g_lp is None and g_ent is None:
+            return None, None, None, None
+        hb, wb, tk, stats, ent = ctx.saved_tensors
+        shape, h_dt, w_dt, temperature = ctx.meta
+        T, V = hb.shape[0], wb.shape[0]
+        gl, ge = _row_grad(g_lp, T), _row_grad(g_ent, T)
+        dh = torch.empty_like(hb)
+        dw = torch.zeros(wb.shape, dtype=F32, device=hb.device)
+        wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
+        with _on_device(hb.device):
+            for lo in range(0, T, LMHeadLogprobsFn.ROWS):
+                hi = min(T, lo + LMHeadLogprobsFn.ROWS)
+                logits = gemm(hb[lo:hi], wb, out_f32=True)
+                call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
+                     ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(logits), _s())
+                dl = logits.to(BF16)
+                if V % 8:
+                    dl = torch.nn.functional.pad(dl, (0, -V % 8))
+                gemm(dl, wp, b_t=True, out=dh[lo:hi])
+                dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True)[:V]
+        return dh.view(shape).to(h_dt), dw.to(w_dt), None, None
+
+
+def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(logprob, entropy) of token_logprobs for the logits hidden [..., d] @ w [V, d]^T, which are never stored
+    whole: memory grows with the tokens, not with tokens times vocabulary.  bf16 operands and fp32 logits as
+    in lm_head_ce; both results are differentiable in hidden and w."""
+    _lib.require_device_tensors("lm_head_logprobs", hidden, w, tokens)
+    _same_device("lm_head_logprobs", hidden, w, tokens)
+    _whole_numbers("lm_head_logprobs", tokens)
+    if w.ndim != 2 or hidden.ndim < 1 or hidden.shape[-1] != w.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"lm_head_logprobs: hidden {tuple(hidden.shape)} and w {tuple(w.shape)} do not match")
+    if tokens.shape != hidden.shape[:-1]:
+        raise ValueError(f"lm_head_logprobs: tokens {tuple(tokens.shape)} do not match hidden {tuple(hidden.shape)}")
+    t = _temperature("lm_head_logprobs", temperature)
+    if fp32_active():
+        return token_logprobs(_f32().linear(hidden, w), tokens, temperature=t)[:2]
+    if w.shape[1] % 8:
+        raise ValueError(f"lm_head_logprobs: the width must be a multiple of 8, got {w.shape[1]}")
+    return LMHeadLogprobsFn.apply(hidden, w, tokens, t)
+
+
+class TopkDistillFn(torch.autograd.Function):
+    """Divergence of rows of logits from a teacher's listed columns (rte_topk_distill_*)."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, temperature: float, tail: bool):
+        dev = logits.device
+        lead, V, K = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
+        lg, ld = _logit_rows(logits)
+        T = lg.shape[0]
+        ic = _ids32(ids.reshape(T, K))
+        tc = teacher.detach().reshape(T, K).contiguous().to(F32)
+        loss = torch.empty((T,), dtype=F32, device=dev)
+        need = ctx.needs_input_grad[0]
+        stats = torch.empty((T, 6), dtype=F32, device=dev) if need else None
+        with _on_device(dev):
+            ws = _scratch(_lib.load().rte_topk_distill_workspace_bytes(T, V, K), dev)
+            call("rte_topk_distill_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), K, temperature,
+                 int(tail), ptr(loss), ptr(stats), ptr(ws), ws.numel(), _s())
+        if need:
+            ctx.save_for_backward(lg, ic, tc, stats)
+            ctx.meta = (logits.shape, ld, temperature, tail)
+        ctx.set_materialize_grads(False)
+        return loss.view(lead)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        if g is None:
+            return (None,) * 5
+        lg, ic, tc, stats = ctx.saved_tensors
+        shape, ld, temperature, tail = ctx.meta
+        T, V = lg.shape
+        gc = _row_grad(g, T)
+        dx = torch.empty((T, V), dtype=lg.dtype, device=lg.device)
+        with _on_device(lg.device):
+            call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), ic.shape[1],
+                 temperature, int(tail), ptr(stats), ptr(gc), ptr(dx), _s())
+        return dx.view(shape), None, None, None, None
+
+
+def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False) -> torch.Tensor:
+    """Per-row divergence temperature^2 KL(teacher || softmax(logits / temperature)) from the columns a teacher
+    kept: logits [..., V] float32 or bfloat16, teacher_ids [..., K] whole numbers and teacher_logits [..., K], K <= 128
+    (token_logprobs' alternatives).  The gradient is the logits' alone.
+
+    tail False: the teacher's distribution is the softmax of its listed logits / temperature (log probabilities
+    do as well).  tail True: teacher_logits are log probabilities at this temperature (token_logprobs(...,
+    temperature=...)), and what they leave of 1 is compared with the student's mass outside the list, so the
+    loss is 0 where both agree on the list and on the rest.
+
+    Negative ids are no entries; of a repeated id the first counts.  A row without entries (tail False: without one above -inf)
+    has loss 0 and no gradient; an id past the vocabulary makes the row's loss NaN and its gradient 0."""
+    _lib.require_device_tensors("topk_distill", logits, teacher_ids, teacher_logits)
+    _same_device("topk_distill", logits, teacher_ids, teacher_logits)
+    _check_logits("topk_distill", logits)
+    _whole_numbers("topk_distill", teacher_ids)
+    if not teacher_logits.is_floating_point():
+        raise TypeError(f"topk_distill: floating-point teacher logits expected, got {teacher_logits.dtype}")
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.ndim < 1 or teacher_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"topk_distill: lists {tuple(teacher_ids.shape)} / {tuple(teacher_logits.shape)} do not match "
+                         f"logits {tuple(logits.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+        raise ValueError(f"topk_distill: lists of 1 to {MAX_TOP} entries expected, got {teacher_ids.shape[-1]}")
+    return TopkDistillFn.apply(logits, teacher_ids, teacher_logits, _temperature("topk_distill", temperature), bool(tail))
 
 
 # ----------------------------------------------------------------------------- audit distillation

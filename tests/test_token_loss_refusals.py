@@ -1,0 +1,60 @@
+"""The C entries of the token losses and the pool balance refuse what they cannot compute, without a device: sizes,
+limits, missing pointers and short workspaces are looked at before anything is launched."""
+
+from __future__ import annotations
+
+import pytest
+
+BUF = 1 << 20  # stands for a device pointer: a refused call never reads it
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from rte_amd import _lib
+
+    return _lib.load()
+
+
+def refused(lib, name, *args):
+    assert getattr(lib, name)(*args) != 0, args
+    assert lib.rte_last_error()
+
+
+def test_token_logprobs(lib):
+    def fwd(x=BUF, ld=64, T=4, V=64, tok=BUF, t=1.0, n=8, lp=BUF, ent=BUF, tl=BUF, ti=BUF, ws=BUF, wsn=1 << 40):
+        refused(lib, "rte_token_logprobs_fwd", x, ld, 1, T, V, tok, t, n, lp, ent, tl, ti, BUF, ws, wsn, None)
+
+    fwd(T=-1), fwd(V=0), fwd(ld=-1), fwd(n=-1), fwd(n=129, V=1000), fwd(n=65), fwd(t=0.0), fwd(t=float("nan"))
+    fwd(t=float("inf")), fwd(x=None), fwd(tok=None), fwd(lp=None), fwd(ent=None), fwd(tl=None), fwd(ti=None)
+    for a in ((None, 64, 1, 4, 64, BUF, 1.0, BUF, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, 1.0, None, BUF, BUF, BUF, BUF),
+              (BUF, 64, 1, 4, 64, BUF, -1.0, BUF, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 0, BUF, 1.0, BUF, BUF, BUF, BUF, BUF),
+              (BUF, 64, 1, 4, 64, BUF, 1.0, BUF, BUF, BUF, BUF, None)):
+        refused(lib, "rte_token_logprobs_bwd", *a, None)
+    assert lib.rte_token_logprobs_fwd(None, 64, 1, 0, 64, None, 1.0, 0, None, None, None, None, None, None, 0, None) == 0
+    assert lib.rte_token_logprobs_bwd(None, 64, 1, 0, 64, None, 1.0, None, None, None, None, None, None) == 0
+
+
+def test_topk_distill(lib):
+    def fwd(x=BUF, ld=64, T=4, V=64, ids=BUF, tl=BUF, K=8, t=1.0, loss=BUF, ws=BUF, wsn=1 << 40):
+        refused(lib, "rte_topk_distill_fwd", x, ld, 1, T, V, ids, tl, K, t, 0, loss, BUF, ws, wsn, None)
+
+    fwd(T=-1), fwd(V=0), fwd(ld=-1), fwd(K=0), fwd(K=129), fwd(t=0.0), fwd(t=float("nan")), fwd(t=float("inf"))
+    fwd(x=None), fwd(ids=None), fwd(tl=None), fwd(loss=None)
+    for a in ((BUF, 64, 1, 4, 64, BUF, BUF, 0, 1.0, 0, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, BUF, 8, 0.0, 0, BUF, BUF, BUF),
+              (BUF, 64, 1, 4, 64, BUF, BUF, 8, 1.0, 0, None, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, BUF, 8, 1.0, 0, BUF, None, BUF)):
+        refused(lib, "rte_topk_distill_bwd", *a, None)
+    assert lib.rte_topk_distill_fwd(None, 64, 1, 0, 64, None, None, 8, 1.0, 0, None, None, None, 0, None) == 0
+
+
+def test_pool_balance(lib):
+    need = lib.rte_pool_balance_workspace_bytes(1000, 64)
+    assert need > 0 and lib.rte_pool_balance_workspace_bytes(0, 64) == 0
+
+    def fwd(x=BUF, ld=64, T=1000, C=64, ids=BUF, k=8, out=BUF, cnt=BUF, frac=BUF, ws=BUF, wsn=need):
+        refused(lib, "rte_pool_balance_fwd", x, ld, 1, T, C, ids, k, None, out, cnt, frac, ws, wsn, None)
+
+    fwd(T=-1), fwd(C=0), fwd(C=1025), fwd(k=0), fwd(ld=-1), fwd(x=None), fwd(ids=None), fwd(out=None), fwd(cnt=None)
+    fwd(frac=None), fwd(ws=None), fwd(wsn=need - 1)
+    refused(lib, "rte_pool_balance_bwd", BUF, 64, 1, 4, 1025, None, BUF, None, None, BUF, None)
+    refused(lib, "rte_pool_balance_bwd", BUF, 64, 1, 4, 64, None, None, None, None, BUF, None)
+    assert lib.rte_pool_balance_bwd(None, 64, 1, 0, 64, None, None, None, None, None, None) == 0
