@@ -648,16 +648,18 @@ int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V
  *           loss = temperature^2 sum_j p_j (log p_j - log q_j)
  *   tail 1: teacher = log probabilities at that temperature, p_j = e^teacher_j, r = max(1 - sum p_j, 0),
  *           loss = temperature^2 (sum_j p_j (log p_j - log q_j) + r (log r - log q(not listed)))
- * A row without entries (tail 0: or without a finite one) has loss 0 and no gradient; an id past the
- * vocabulary makes the loss NaN and the gradient 0.  K <= 128.  stats f32 [T, 6], NULL without a backward.
+ * A row without entries (tail 0: or without one above -inf) has loss 0 and no gradient; an id past the
+ * vocabulary makes the loss NaN and the gradient 0.  K <= 128.
+ * Kept for the backward (stats NULL: nothing is): stats f32 [T, 2], cols int32 [T, K] = the columns that count
+ * (-1: none), coef f32 [T, K] = q - p there.
  * bwd: dlogits [T, V] dense in the logits' type, for g f32 [T]. */
 size_t rte_topk_distill_workspace_bytes(int T, int V, int K);
 int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
                          const float* teacher, int K, float temperature, int tail, float* loss, float* stats,
-                         void* workspace, size_t workspace_bytes, void* stream);
-int rte_topk_distill_bwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
-                         const float* teacher, int K, float temperature, int tail, const float* stats,
-                         const float* g, void* dlogits, void* stream);
+                         int32_t* cols, float* coef, void* workspace, size_t workspace_bytes, void* stream);
+int rte_topk_distill_bwd(const void* logits, int64_t ld, int f32, int T, int V, int K, float temperature,
+                         const float* stats, const int32_t* cols, const float* coef, const float* g,
+                         void* dlogits, void* stream);
 
 /* ---- hot-vs-exact distillation losses + alignment metrics of the audit (replaces
  *      macro_distill_loss rte/macro.py:394-471 and macro_alignment_metrics :499-546 on the

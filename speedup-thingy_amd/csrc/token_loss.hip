@@ -19,229 +19,708 @@ namespace rte {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMaxTop = 128;  // alternatives or list entries per row
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-__device__ __forceinline__ float logit(const float* x, int64_t i) { return x[i]; }
-__device__ __forceinline__ float logit(const bf16* x, int64_t i) { return bf2f(x[i]); }
-__device__ __forceinline__ void put(float* x, int64_t i, float v) { x[i] = v; }
-__device__ __forceinline__ void put(bf16* x, int64_t i, float v) { x[i] = f2bf(v); }
+// Sixteen bytes of a row at any alignment of its element type: rows of odd length start anywhere, and a
+// global load or store of four words asks for no more.
+typedef uint32_t words_v __attribute__((ext_vector_type(4), aligned(2), may_alias));
+struct Words {
+  uint32_t w[4];
+};
+
+template <class X>
+struct Row;
+template <>
+struct Row<float> {
+  static constexpr int VE = 4;
+  __device__ static float one(const float* x, int64_t i) { return x[i]; }
+  __device__ static void put(float* x, int64_t i, float v) { x[i] = v; }
+  __device__ static float get(const Words& v, int j) { return __uint_as_float(v.w[j]); }
+  __device__ static void set(Words& v, int j, float f) { v.w[j] = __float_as_uint(f); }
+  __device__ static Words pack(const float* f) {
+    return {{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}};
+  }
+};
+template <>
+struct Row<bf16> {
+  static constexpr int VE = 8;
+  __device__ static float one(const bf16* x, int64_t i) { return bf2f(x[i]); }
+  __device__ static void put(bf16* x, int64_t i, float v) { x[i] = f2bf(v); }
+  __device__ static float get(const Words& v, int j) {
+    return __uint_as_float(j & 1 ? v.w[j >> 1] & 0xffff0000u : v.w[j >> 1] << 16);
+  }
+  __device__ static void set(Words& v, int j, float f) {
+    const uint32_t h = __float_as_uint(f) >> 16;
+    v.w[j >> 1] = j & 1 ? (v.w[j >> 1] & 0xffffu) | h << 16 : (v.w[j >> 1] & 0xffff0000u) | h;
+  }
+  __device__ static Words pack(const float* f) {
+    return {{pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7])}};
+  }
+};
+
+// Elements at .. at + VE of a row that ends at `end`; what lies past the end is -inf.
+template <class X>
+__device__ __forceinline__ Words load_words(const X* row, int at, int end) {
+  constexpr int VE = Row<X>::VE;
+  Words r;
+  if (at + VE <= end) {
+    const words_v v = *reinterpret_cast<const words_v*>(row + at);
+    r = {{v.x, v.y, v.z, v.w}};
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) Row<X>::set(r, j, at + j < end ? Row<X>::one(row, at + j) : -INFINITY);
+  }
+  return r;
+}
+
+template <class X>
+__device__ __forceinline__ void store_words(X* row, int at, int end, const float* f) {
+  constexpr int VE = Row<X>::VE;
+  if (at + VE <= end) {
+    const Words p = Row<X>::pack(f);
+    *reinterpret_cast<words_v*>(row + at) = words_v{p.w[0], p.w[1], p.w[2], p.w[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      if (at + j < end) Row<X>::put(row, at + j, f[j]);
+  }
+}
 
 // Order of the alternatives as unsigned keys: larger value first, -0 = +0, NaN above everything.
+constexpr uint32_t kNanKey = 0xfffffffeu, kInfKey = 0xff800000u;
+typedef unsigned long long u64;
 __device__ __forceinline__ uint32_t value_key(float x) {
-  if (x != x) return 0xfffffffeu;
   const uint32_t b = __float_as_uint(x + 0.0f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return x != x ? kNanKey : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k > kInfKey ? 0x7fc00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ u64 full_key(float x, int col) { return (u64)value_key(x) << 32 | (uint32_t)~col; }
 
-template <class F>
-__device__ __forceinline__ float block_reduce(float v, F f, float* red) {
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <class V>
+__device__ __forceinline__ V wave_sum(V v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < kThreads / 64; ++i) v = f(v, red[i]);
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-struct Max {
-  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+template <class V>
+__device__ __forceinline__ V wave_max(V v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const V u = __shfl_xor(v, o, 64);
+    v = u > v || v != v ? u : v;  // NaN loses
+  }
+  return v;
+}
+
+struct RowArgs {
+  int64_t ld;
+  int T, V;
+  int nparts, part;  // a row is computed in nparts ranges of `part` columns
+  float c2, inv_t;   // log2(e) / t, 1 / t
+  // log probabilities
+  const int64_t* tokens;
+  int n_top;
+  float *logprob, *entropy, *top_lp;
+  int32_t* top_ids;
+  // divergence
+  const int32_t* ids;
+  const float* tl;
+  int K, tail;
+  double it, t2;
+  float* loss;
+  int32_t* cols;
+  float* coef;
+  float* stats;       // kept for the backward (NULL: none)
+  float4* part_stats; // [T, nparts] {max, sum, sum of e u}
+  u64* part_keys;     // [T, nparts, n_top]
 };
-struct Sum {
-  __device__ float operator()(float a, float b) const { return a + b; }
+
+// One row's sums, relative to its maximum m: s = sum e^u, su = log2(e) sum e^u u with u = (x - m) / t.
+struct Sums {
+  float m, s, su;
 };
 
 template <class X>
-__global__ void __launch_bounds__(kThreads)
-    logprobs_fwd_kernel(const X* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
-                        float inv_t, int n_top, float* __restrict__ logprob, float* __restrict__ entropy,
-                        float* __restrict__ top_lp, int32_t* __restrict__ top_ids, float* __restrict__ stats) {
-  __shared__ float red[kThreads / 64];
-  __shared__ unsigned long long best[kThreads / 64];
-  const int64_t t = blockIdx.x;
-  const X* row = logits + t * ld;
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < V; v += kThreads) m = fmaxf(m, logit(row, v));
-  m = block_reduce(m, Max(), red);
-  const bool none = m == -INFINITY;  // no column is possible (a row of NaN keeps its NaN through S)
-  float s = 0.0f, su = 0.0f;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    const float u = (logit(row, v) - (none ? 0.0f : m)) * inv_t;
-    const float e = __expf(u);
-    s += e;
-    su += e * fmaxf(u, -200.0f);
+__device__ __forceinline__ void finish_logprobs(const RowArgs& a, const X* row, int64_t t, const Sums& r) {
+  const int64_t tok = a.tokens[t];
+  const float log_s = logf(r.s);
+  const bool empty = r.s == 0.0f;  // no column above -inf
+  float lp = 0.0f;
+  if (tok >= a.V) lp = __builtin_nanf("");
+  else if (tok >= 0) lp = empty ? -INFINITY : (Row<X>::one(row, tok) - r.m) * a.inv_t - log_s;
+  a.logprob[t] = lp;
+  a.entropy[t] = empty ? 0.0f : log_s - r.su * kLn2 / r.s;
+  if (a.stats) {
+    a.stats[2 * t] = r.m;
+    a.stats[2 * t + 1] = log_s;
   }
-  s = block_reduce(s, Sum(), red);
-  su = block_reduce(su, Sum(), red);
-  const bool empty = none && s == 0.0f;
-  const float log_s = logf(s);
-  if (threadIdx.x == 0) {
-    const int64_t tok = tokens[t];
-    float lp = 0.0f;
-    if (tok >= V) lp = __builtin_nanf("");
-    else if (tok >= 0) lp = empty ? -INFINITY : (logit(row, tok) - m) * inv_t - log_s;
-    logprob[t] = lp;
-    entropy[t] = empty ? 0.0f : log_s - su / s;
-    if (stats) {
-      stats[2 * t] = m;
-      stats[2 * t + 1] = log_s;
-    }
+}
+
+__device__ __forceinline__ void put_top(const RowArgs& a, int64_t t, int rank, u64 key, const Sums& r) {
+  a.top_ids[t * a.n_top + rank] = (int32_t)~(uint32_t)key;
+  a.top_lp[t * a.n_top + rank] =
+      r.s == 0.0f ? -INFINITY : (key_value((uint32_t)(key >> 32)) - r.m) * a.inv_t - logf(r.s);
+}
+
+// The divergence of row t by one wave, from the sums of the columns not listed (rest.m = -inf: none).
+// Lane i holds entries i and i + 64.  The list's part is computed in 64 bits: for a student near its teacher
+// the terms p (log p - log q) cancel to the square of the difference, and q's total is put together from the
+// same list and rest, so that an error of the rest's sum enters multiplied by that difference.  `unique`: no
+// column is listed twice.
+// Kept for the backward: dx_v = g t coef_j at column cols_j, g t c e^{(x_v - m) / t} elsewhere, with {m, c}
+// in stats (c = 0: the row has no gradient).
+template <class X>
+__device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const Sums& rest, bool unique, int lane) {
+  const int32_t* ids = a.ids + t * a.K;
+  const float* tl = a.tl + t * a.K;
+  int col[2];
+  float y[2];
+  double x[2];
+  bool foreign = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 64 * i;
+    col[i] = j < a.K ? ids[j] : -1;
+    y[i] = j < a.K ? tl[j] : 0.0f;
+    foreign |= col[i] >= a.V;
   }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < n_top; ++j) {
-    unsigned long long top = 0;
-    for (int v = threadIdx.x; v < V; v += kThreads) {
-      const unsigned long long key = (unsigned long long)value_key(logit(row, v)) << 32 | (uint32_t)~v;
-      if (key < last && key > top) top = key;
+  if (!unique) {
+    bool again[2] = {false, false};
+    for (int j = 0; j < a.K; ++j) {
+      const int c = __shfl(col[j >> 6], j & 63, 64);
+      again[0] |= c == col[0] && j < lane;
+      again[1] |= c == col[1] && j < lane + 64;
     }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const unsigned long long other = __shfl_xor(top, o, 64);
-      top = other > top ? other : top;
+    for (int i = 0; i < 2; ++i)
+      if (again[i]) col[i] = -1;
+  }
+  foreign = __any(foreign);
+  double top = rest.m, tmax = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (col[i] >= a.V) col[i] = -1;
+    x[i] = col[i] >= 0 ? (double)Row<X>::one(row, col[i]) : -INFINITY;
+    if (col[i] >= 0) tmax = y[i] > tmax || tmax != tmax ? y[i] : tmax;
+    top = x[i] > top || top != top ? x[i] : top;
+  }
+  bool some = __any(col[0] >= 0 || col[1] >= 0);
+  top = wave_max(top);
+  tmax = wave_max(tmax);
+  // NaN entries reach the sums; a list of -inf alone holds no probability
+  const bool teacher_nan = __any((col[0] >= 0 && y[0] != y[0]) || (col[1] >= 0 && y[1] != y[1]));
+  if (!a.tail && tmax == -INFINITY && !teacher_nan) some = false;
+  const double m = top == -INFINITY ? 0.0 : top;
+  const double scale = rest.m == -INFINITY ? 0.0 : exp(((double)rest.m - m) * a.it);
+  double rsum = rest.s == 0.0f ? 0.0 : rest.s * scale;  // a NaN sum stays
+  if (rest.m == -INFINITY && rest.s != 0.0f) rsum = __builtin_nan("");
+  double e[2], p[2], lp[2], total = 0.0, tsum = 0.0, psum = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e[i] = col[i] >= 0 ? exp((x[i] - m) * a.it) : 0.0;
+    total += e[i];
+    lp[i] = a.tail ? (double)y[i] : ((double)y[i] - (tmax == -INFINITY ? 0.0 : tmax)) * a.it;
+    p[i] = col[i] >= 0 ? exp(lp[i]) : 0.0;
+    tsum += p[i];
+  }
+  total = wave_sum(total) + rsum;
+  tsum = wave_sum(tsum);
+  const double log_s = log(total);
+  if (!a.tail) {
+    const double tlog = log(tsum), inv = 1.0 / tsum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lp[i] -= tlog;
+      p[i] *= inv;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < kThreads / 64; ++i) top = best[i] > top ? best[i] : top;
-    last = top;
-    if (threadIdx.x == 0) {
-      const int v = (int)~(uint32_t)top;
-      top_ids[t * n_top + j] = v;
-      top_lp[t * n_top + j] = empty ? -INFINITY : (logit(row, v) - m) * inv_t - log_s;
-    }
+    psum = 1.0;
+  } else {
+    psum = tsum;
   }
-}
-
-template <class X>
-__global__ void __launch_bounds__(kThreads)
-    logprobs_bwd_kernel(const X* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
-                        float inv_t, const float* __restrict__ stats, const float* __restrict__ entropy,
-                        const float* __restrict__ g_lp, const float* __restrict__ g_ent, X* __restrict__ dlogits) {
-  const int64_t t = blockIdx.x;
-  const X* row = logits + t * ld;
-  X* out = dlogits + t * V;
-  const float m = stats[2 * t], log_s = stats[2 * t + 1], h = entropy[t];
-  const int64_t tok = tokens[t];
-  const float g = g_lp && tok >= 0 && tok < V ? g_lp[t] : 0.0f, gh = g_ent ? g_ent[t] : 0.0f;
-  const bool empty = log_s == -INFINITY;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    const float lp = (logit(row, v) - m) * inv_t - log_s;
-    const float d = (v == tok ? g : 0.0f) - __expf(lp) * (g + gh * (fmaxf(lp, -200.0f) + h));
-    put(out, v, empty ? 0.0f : d * inv_t);
-  }
-}
-
-// Row statistics of the divergence, kept for the backward: {max, log S of the whole row (relative to max),
-// log of the teacher's normaliser (tail 0: of e^{(t_j - max t) / t}), the teacher's rest r}, then the
-// rest's log sum relative to max.
-constexpr int kDistillStats = 6;
-enum { D_MAX, D_LOGS, D_TMAX, D_TLOG, D_REST, D_LOGR };
-
-// Whether entry j is the first of its column and inside the vocabulary.
-__device__ __forceinline__ bool counts(const int32_t* ids, int j, int V) {
-  const int c = ids[j];
-  if (c < 0 || c >= V) return false;
-  for (int i = 0; i < j; ++i)
-    if (ids[i] == c) return false;
-  return true;
-}
-
-template <class X>
-__global__ void __launch_bounds__(kThreads)
-    distill_fwd_kernel(const X* __restrict__ logits, int64_t ld, int V, const int32_t* __restrict__ ids,
-                       const float* __restrict__ tl, int K, float temp, int tail, float* __restrict__ loss,
-                       float* __restrict__ stats) {
-  __shared__ float red[kThreads / 64];
-  __shared__ uint8_t first[kMaxTop];
-  const int64_t t = blockIdx.x;
-  const X* row = logits + t * ld;
-  ids += t * K;
-  tl += t * K;
-  const float inv_t = 1.0f / temp;
-  if (threadIdx.x < K) first[threadIdx.x] = counts(ids, threadIdx.x, V);
-  __syncthreads();
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < V; v += kThreads) m = fmaxf(m, logit(row, v));
-  m = block_reduce(m, Max(), red);
-  const bool none = m == -INFINITY;
-  const float m0 = none ? 0.0f : m;
-  float s = 0.0f;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    bool listed = false;
-    for (int j = 0; j < K; ++j) listed |= ids[j] == v;
-    s += listed ? 0.0f : __expf((logit(row, v) - m0) * inv_t);
-  }
-  s = block_reduce(s, Sum(), red);
-  if (threadIdx.x != 0) return;
-  bool bad = false, some = false;
-  double tmax = -INFINITY;
-  for (int j = 0; j < K; ++j) {
-    bad |= ids[j] >= V;
-    if (!first[j]) continue;
-    some = true;
-    tmax = fmax(tmax, (double)tl[j]);
-  }
-  if (!tail && tmax == -INFINITY) some = false;  // the list holds no probability
-  const double it = 1.0 / (double)temp;
-  double rest = s, total = rest, tsum = 0.0, psum = 0.0;
-  for (int j = 0; j < K; ++j) {
-    if (!first[j]) continue;
-    total += exp(((double)logit(row, ids[j]) - m0) * it);
-    tsum += exp(((double)tl[j] - tmax) * it);
-  }
-  const double log_s = log(total), tlog = log(tsum);
   const bool empty = total == 0.0;
   double l = 0.0;
-  for (int j = 0; j < K; ++j) {
-    if (!first[j]) continue;
-    const double lp = tail ? (double)tl[j] : ((double)tl[j] - tmax) * it - tlog;
-    const double lq = empty ? -INFINITY : ((double)logit(row, ids[j]) - m0) * it - log_s;
-    const double p = exp(lp);
-    psum += p;
-    if (p > 0.0 || lp != lp) l += p * (lp - lq);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double lq = empty ? -INFINITY : (x[i] - m) * a.it - log_s;
+    if (col[i] >= 0 && p[i] != 0.0) l += p[i] * (lp[i] - lq);
   }
-  double r = tail ? fmax(1.0 - psum, 0.0) : 0.0;
-  if (r > 0.0) l += r * (log(r) - (empty ? -INFINITY : log(rest) - log_s));
-  if (bad) l = __builtin_nan("");
-  loss[t] = some || bad ? (float)(l * temp * temp) : 0.0f;
-  if (stats) {
-    stats += t * kDistillStats;
-    stats[D_MAX] = m0;
-    stats[D_LOGS] = (float)log_s;
-    stats[D_TMAX] = some && !bad ? (float)tmax : __builtin_nanf("");
-    stats[D_TLOG] = (float)tlog;
-    stats[D_REST] = (float)r;
-    stats[D_LOGR] = (float)log(rest);
+  l = wave_sum(l);
+  const double r = a.tail ? (psum > 1.0 ? 0.0 : 1.0 - psum) : 0.0;
+  if (r > 0.0) l += r * (log(r) - (empty ? -INFINITY : log(rsum) - log_s));
+  if (lane == 0) a.loss[t] = foreign ? __builtin_nanf("") : some ? (float)(l * a.t2) : 0.0f;
+  if (!a.stats) return;
+  const bool none = foreign || !some || empty;
+  const double inv = 1.0 / total;
+  if (lane == 0) {
+    const bool out = none || (rsum == 0.0 && rest.m == -INFINITY);
+    a.stats[2 * t] = out ? 0.0f : rest.m;
+    // (q(R) - r) / (the rest's sum relative to its own maximum)
+    a.stats[2 * t + 1] = out ? 0.0f : (float)((rsum * inv - r) / rest.s);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 64 * i;
+    if (j >= a.K) continue;
+    a.cols[t * a.K + j] = none ? -1 : col[i];
+    a.coef[t * a.K + j] = none ? 0.0f : (float)(e[i] * inv - p[i]);
   }
 }
 
-template <class X>
-__global__ void __launch_bounds__(kThreads)
-    distill_bwd_kernel(const X* __restrict__ logits, int64_t ld, int V, const int32_t* __restrict__ ids,
-                       const float* __restrict__ tl, int K, float temp, int tail, const float* __restrict__ stats,
-                       const float* __restrict__ g, X* __restrict__ dlogits) {
-  const int64_t t = blockIdx.x;
-  const X* row = logits + t * ld;
-  X* out = dlogits + t * V;
-  ids += t * K;
-  tl += t * K;
-  stats += t * kDistillStats;
-  const float inv_t = 1.0f / temp, gt = g[t] * temp;
-  const float m = stats[D_MAX], log_s = stats[D_LOGS], r = stats[D_REST], log_r = stats[D_LOGR];
-  const float tmax = stats[D_TMAX], tlog = stats[D_TLOG];
-  const bool skip = tmax != tmax || log_s == -INFINITY;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    int at = -1;
-    for (int j = K - 1; j >= 0; --j)
-      if (ids[j] == v) at = j;
-    const float u = (logit(row, v) - m) * inv_t;
-    float d = __expf(u - log_s);
-    if (at >= 0) d -= __expf(tail ? tl[at] : (tl[at] - tmax) * inv_t - tlog);
-    else if (r > 0.0f) d -= r * __expf(u - log_r);
-    put(out, v, skip ? 0.0f : gt * d);
+// Threads that share a row (or a range of one): one wave, or the four of a workgroup.
+template <int NW>
+struct Group {
+  static constexpr int NT = 64 * NW;
+  float* red;  // [3 * NW]
+  int tid, wave;
+  __device__ __forceinline__ void sync() const {
+    if constexpr (NW == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  }
+  // total of a per-wave count (uniform in the wave)
+  __device__ int count(int n) const {
+    if constexpr (NW == 1) return n;
+    __syncthreads();
+    if ((tid & 63) == 0) reinterpret_cast<int*>(red)[wave] = n;
+    __syncthreads();
+    int s = 0;
+    for (int i = 0; i < NW; ++i) s += reinterpret_cast<int*>(red)[i];
+    return s;
+  }
+};
+
+constexpr int kRowCols = 2048;  // columns of a row that one wave holds
+constexpr int kCandWave = 512, kCandGroup = 1024;
+
+// One pass over a row (or one of its ranges), held in registers: E columns per thread.  The maximum comes
+// first, so no sum is rescaled.  For the alternatives, the n-th largest of 256 maxima (of a thread's
+// columns, or quarters of them) is a threshold that n columns reach at least; those that do, about n ln(...)
+// of them, go to LDS and each finds its rank there by counting.  Rows whose ties bring more than LDS holds
+// find the n-th value and the last of its columns by bits.
+template <class X, int NW, int E, bool DIST, bool TOP>
+__global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ logits, RowArgs a) {
+  constexpr int VE = Row<X>::VE, NV = E / VE, NT = 64 * NW, GROUPS = 4 / NW, RPB = 4 / NW;
+  constexpr int CAP = NW == 1 ? kCandWave : kCandGroup;
+  constexpr int MASKW = NT * E / 32;
+  static_assert(NV * VE == E && NV >= GROUPS && NV % GROUPS == 0, "whole vectors, a group of them each");
+  __shared__ float s_red[RPB][3 * NW];
+  __shared__ uint32_t s_mask[DIST ? RPB : 1][DIST ? MASKW : 1];
+  __shared__ u64 s_cand[TOP ? RPB : 1][TOP ? CAP + 2 : 1];
+  __shared__ uint32_t s_gmax[TOP && NW > 1 ? 256 : 1];
+  __shared__ int s_ctl[2];  // candidates, threshold
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slot = NW == 1 ? wave : 0;
+  Group<NW> grp{s_red[slot], NW == 1 ? lane : (int)threadIdx.x, NW == 1 ? 0 : wave};
+  const int tid = grp.tid;
+  int64_t t;
+  int p = 0;
+  if constexpr (NW == 1) {
+    t = (int64_t)blockIdx.x * 4 + wave;
+    if (t >= a.T) return;
+  } else {
+    t = blockIdx.x / (unsigned)a.nparts;
+    p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
+  }
+  const X* row = logits + t * a.ld;
+  const int c0 = p * a.part;
+  const int len = a.V - c0 < a.part ? a.V - c0 : a.part;
+  const X* at = row + c0;
+
+  Words w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int off = (i * NT + tid) * VE;
+    if (i * NT * VE < len) {
+      w[i] = load_words(at, off, len);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) Row<X>::set(w[i], j, -INFINITY);
+    }
+  }
+
+  bool unique = true;
+  if constexpr (DIST) {
+    uint32_t* mask = s_mask[slot];
+    for (int i = tid; i < MASKW; i += NT) mask[i] = 0;
+    grp.sync();
+    bool again = false;
+    for (int j = tid; j < a.K; j += NT) {
+      const int id = a.ids[t * a.K + j], rel = id - c0;
+      if (id >= c0 && rel < len) again |= (atomicOr(&mask[rel >> 5], 1u << (rel & 31)) >> (rel & 31)) & 1;
+    }
+    unique = !__any(again);  // as far as this wave sees: of NW > 1, entries 64 wave .. 64 wave + 63
+    grp.sync();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int off = (i * NT + tid) * VE;
+      const uint32_t bits = mask[off >> 5] >> (off & 31) & ((1u << VE) - 1);
+      if (bits) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (bits >> j & 1) Row<X>::set(w[i], j, -INFINITY);
+      }
+    }
+  }
+
+  // maxima (a NaN column shows in the sums)
+  float gm[GROUPS];
+  uint32_t gk[GROUPS];
+  float m = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    gm[g] = -INFINITY;
+#pragma unroll
+    for (int i = g * (NV / GROUPS); i < (g + 1) * (NV / GROUPS); ++i)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) gm[g] = fmaxf(gm[g], Row<X>::get(w[i], j));
+    m = fmaxf(m, gm[g]);
+    gk[g] = value_key(gm[g]);
+  }
+  m = wave_max(m);
+  if constexpr (NW > 1) {
+    if (lane == 0) grp.red[wave] = m;
+    if constexpr (TOP) s_gmax[tid] = gk[0];
+    if (tid == 0) s_ctl[0] = 0;
+    __syncthreads();
+    m = fmaxf(fmaxf(grp.red[0], grp.red[1]), fmaxf(grp.red[2], grp.red[3]));
+  }
+
+  // threshold: the want-th largest of 256 maxima, to the leading bits (16 of them are all of a bf16 value)
+  const int want = a.n_top;
+  uint32_t thr = 0;
+  if constexpr (TOP) {
+    if (NW == 1 || wave == 0) {
+      uint32_t k[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if constexpr (NW == 1) k[g] = gk[g];
+        else k[g] = s_gmax[lane + 64 * g];
+      }
+      for (int b = 31; b >= (VE == 8 ? 16 : 12); --b) {
+        const uint32_t c = thr | 1u << b;
+        int n = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) n += __popcll(__ballot(k[g] >= c));
+        if (n >= want) thr = c;
+        if (n == want) break;
+      }
+      if constexpr (NW > 1) {
+        if (lane == 0) s_ctl[1] = (int)thr;
+      }
+    }
+  }
+
+  const float m0 = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f, su = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float u = (Row<X>::get(w[i], j) - m0) * a.c2;
+      const float e = exp2_(u);
+      s += e;
+      if constexpr (!DIST) su += e * fmaxf(u, -256.0f);  // -inf: e is 0 and the product has to be
+    }
+  s = wave_sum(s);
+  if constexpr (!DIST) su = wave_sum(su);
+  if constexpr (NW > 1) {
+    if (lane == 0) {
+      grp.red[NW + wave] = s;
+      grp.red[2 * NW + wave] = su;
+    }
+    __syncthreads();
+    s = (grp.red[NW] + grp.red[NW + 1]) + (grp.red[NW + 2] + grp.red[NW + 3]);
+    su = (grp.red[2 * NW] + grp.red[2 * NW + 1]) + (grp.red[2 * NW + 2] + grp.red[2 * NW + 3]);
+    if constexpr (TOP) thr = (uint32_t)s_ctl[1];
+  }
+  const Sums r{m, s, su};
+
+  if (NW > 1 && a.nparts > 1) {
+    if (tid == 0) a.part_stats[t * a.nparts + p] = make_float4(m, s, su, 0.0f);
+  } else if constexpr (DIST) {
+    if (NW == 1 || wave == 0) finish_distill(a, row, t, r, unique && (NW == 1 || a.K <= 64), lane);
+  } else {
+    if (tid == 0) finish_logprobs(a, row, t, r);
+  }
+
+  if constexpr (TOP) {
+    u64* cand = s_cand[slot];
+    const float least = key_value(thr);  // not less than it: in (NaN and, where it is NaN, everything in)
+    int n = 0;
+    auto collect = [&](auto in) {
+      n = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int off = (i * NT + tid) * VE;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const float x = Row<X>::get(w[i], j);
+          const bool here = in(x, off + j) && off + j < len;
+          const u64 who = __ballot(here);
+          if (who == 0) continue;
+          int base = n;
+          if constexpr (NW > 1) {
+            if (lane == 0) base = atomicAdd(&s_ctl[0], __popcll(who));
+            base = __builtin_amdgcn_readfirstlane(base);
+          }
+          const int pos = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+          if (here && pos < CAP) cand[pos] = full_key(x, c0 + off + j);
+          n += __popcll(who);
+        }
+      }
+      grp.sync();
+      if constexpr (NW > 1) n = s_ctl[0];
+    };
+    collect([&](float x, int) { return !(x < least); });
+    if (n > CAP) {
+      // value of rank `want`, then the last of its columns that is in
+      auto total = [&](auto in) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          // a row's keys are made again for every bit: hoisted, they took 241 registers where the row takes 32
+          asm volatile("" : "+v"(w[i].w[0]), "+v"(w[i].w[1]), "+v"(w[i].w[2]), "+v"(w[i].w[3]));
+#pragma unroll
+          for (int j = 0; j < VE; ++j) {
+            const int rel = (i * NT + tid) * VE + j;
+            c += __popcll(__ballot(rel < len && in(value_key(Row<X>::get(w[i], j)), rel)));
+          }
+        }
+        return grp.count(c);
+      };
+      uint32_t kth = 0;
+      for (int b = 31; b >= 0; --b) {
+        const uint32_t c = kth | 1u << b;
+        if (total([&](uint32_t k, int) { return k >= c; }) >= want) kth = c;
+      }
+      const int need = want - total([&](uint32_t k, int) { return k > kth; });
+      int last = 0;
+      for (int b = 13; b >= 0; --b) {
+        const int c = last | 1 << b;
+        if (total([&](uint32_t k, int rel) { return k == kth && rel < c; }) < need) last = c;
+      }
+      if (NW > 1) {
+        __syncthreads();
+        if (tid == 0) s_ctl[0] = 0;
+        __syncthreads();
+      }
+      collect([&](float x, int rel) {
+        const uint32_t k = value_key(x);
+        return k > kth || (k == kth && rel <= last);
+      });
+    }
+    if (tid < 2) cand[n + tid] = 0;
+    grp.sync();
+    for (int c = tid; c < n; c += NT) {
+      const u64 mine = cand[c];
+      int rank = 0;
+      for (int j = 0; j < n; j += 2) rank += (cand[j] > mine) + (cand[j + 1] > mine);
+      if (rank >= want) continue;
+      if (NW > 1 && a.nparts > 1) a.part_keys[(t * a.nparts + p) * want + rank] = mine;
+      else put_top(a, t, rank, mine, r);
+    }
+    if (NW > 1 && a.nparts > 1)  // a short last range
+      for (int c = n + tid; c < want; c += NT) a.part_keys[(t * a.nparts + p) * want + c] = 0;
   }
 }
+
+// Joins a row's ranges: sums rescaled to the common maximum, the alternatives merged by rank (a key's rank is
+// the number of larger keys in every range's sorted list).
+constexpr int kJoinKeys = 2048;
+template <class X, bool DIST, bool TOP>
+__global__ void __launch_bounds__(TOP ? 256 : 64) rows_join_kernel(const X* __restrict__ logits, RowArgs a) {
+  __shared__ u64 s_keys[TOP ? kJoinKeys : 1];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const float4* part = a.part_stats + t * a.nparts;
+  float m = -INFINITY;
+  for (int i = lane; i < a.nparts; i += 64) m = fmaxf(m, part[i].x);
+  m = wave_max(m);
+  const float m0 = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f, su = 0.0f;
+  for (int i = lane; i < a.nparts; i += 64) {
+    const float4 q = part[i];
+    const float u = (q.x - m0) * a.c2, e = exp2_(u);
+    s += q.y != q.y ? q.y : q.y * e;
+    su += e * (q.z + q.y * fmaxf(u, -256.0f));
+  }
+  const Sums r{m, wave_sum(s), wave_sum(su)};
+  const X* row = logits + t * a.ld;
+  if constexpr (DIST) {
+    finish_distill(a, row, t, r, false, lane);
+  } else {
+    if (threadIdx.x == 0) finish_logprobs(a, row, t, r);
+  }
+  if constexpr (TOP) {
+    const int K = a.n_top, n = a.nparts * K;
+    const u64* keys = a.part_keys + t * n;
+    const bool fits = n <= kJoinKeys;
+    if (fits) {
+      for (int i = threadIdx.x; i < n; i += 256) s_keys[i] = keys[i];
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const u64 mine = fits ? s_keys[i] : keys[i];
+      if (mine == 0) continue;
+      int rank = 0;
+      for (int q = 0; q < a.nparts && rank < K; ++q) {
+        int lo = 0, hi = K;  // keys of list q above mine
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          const u64 o = fits ? s_keys[q * K + mid] : keys[q * K + mid];
+          if (o > mine) lo = mid + 1;
+          else hi = mid;
+        }
+        rank += lo;
+      }
+      if (rank < K) put_top(a, t, rank, mine, r);
+    }
+  }
+}
+
+constexpr int kSeg = 2048;  // columns of a wave in the backward passes
+
+template <class X>
+__global__ void __launch_bounds__(256)
+    logprobs_bwd_kernel(const X* __restrict__ logits, int64_t ld, int64_t items, int V, int nseg,
+                        const int64_t* __restrict__ tokens, float inv_t, const float* __restrict__ stats,
+                        const float* __restrict__ entropy, const float* __restrict__ g_lp,
+                        const float* __restrict__ g_ent, X* __restrict__ dlogits) {
+  constexpr int VE = Row<X>::VE, NV = kSeg / 64 / VE;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= items) return;
+  const int64_t t = item / nseg;
+  const int c0 = (int)(item - t * nseg) * kSeg;
+  const int len = V - c0 < kSeg ? V - c0 : kSeg;
+  const X* x = logits + t * ld + c0;
+  X* out = dlogits + t * V + c0;
+  Words w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * 64) * VE < len) w[i] = load_words(x, (i * 64 + lane) * VE, len);
+  const float m = stats[2 * t], log_s = stats[2 * t + 1];
+  const int64_t tok = tokens[t];
+  const float g = g_lp && tok >= 0 && tok < V ? g_lp[t] : 0.0f, gh = g_ent ? g_ent[t] : 0.0f;
+  const float gc = g + gh * entropy[t];
+  const bool empty = log_s == -INFINITY;
+  // the token's column is written again by the lane that holds it
+  const int64_t rel = tok - c0;
+  const bool mine = g != 0.0f && !empty && rel >= 0 && rel < len && (int)(rel / VE) % 64 == lane;
+  const float at_tok = mine ? Row<X>::one(x, rel) : 0.0f;
+  auto slope = [&](float v) {  // of every column: -p (g + g_H (log p + H)) / t
+    const float lp = (v - m) * inv_t - log_s;
+    return -exp2_(lp * kLog2e) * (gc + gh * fmaxf(lp, -200.0f)) * inv_t;
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i * 64) * VE >= len) continue;
+    float d[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) d[j] = empty ? 0.0f : slope(Row<X>::get(w[i], j));
+    store_words(out, (i * 64 + lane) * VE, len, d);
+  }
+  if (mine) Row<X>::put(out, rel, slope(at_tok) + g * inv_t);
+}
+
+template <class X>
+__global__ void __launch_bounds__(256)
+    distill_bwd_kernel(const X* __restrict__ logits, int64_t ld, int64_t items, int V, int nseg, int K, float c2,
+                       float temp, const float* __restrict__ stats, const int32_t* __restrict__ cols,
+                       const float* __restrict__ coef, const float* __restrict__ g, X* __restrict__ dlogits) {
+  constexpr int VE = Row<X>::VE, NV = kSeg / 64 / VE;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= items) return;
+  const int64_t t = item / nseg;
+  const int c0 = (int)(item - t * nseg) * kSeg;
+  const int len = V - c0 < kSeg ? V - c0 : kSeg;
+  const X* x = logits + t * ld + c0;
+  X* out = dlogits + t * V + c0;
+  Words w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * 64) * VE < len) w[i] = load_words(x, (i * 64 + lane) * VE, len);
+  int col[2];
+  float cf[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 64 * i;
+    col[i] = j < K ? cols[t * K + j] - c0 : -1;
+    cf[i] = j < K ? coef[t * K + j] : 0.0f;
+  }
+  const float m = stats[2 * t], gt = g[t] * temp, c = stats[2 * t + 1] * gt;
+  const bool none = stats[2 * t + 1] == 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i * 64) * VE >= len) continue;
+    float d[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) d[j] = none ? 0.0f : c * exp2_((Row<X>::get(w[i], j) - m) * c2);
+    store_words(out, (i * 64 + lane) * VE, len, d);
+  }
+  // the listed columns, once every lane's stores are done
+  const bool here[2] = {col[0] >= 0 && col[0] < len, col[1] >= 0 && col[1] < len};
+  if (!__any(here[0] || here[1])) return;
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (here[i]) Row<X>::put(out, col[i], gt * cf[i]);
+}
+
+// Ranges of a row.  One wave holds up to 2048 columns, a workgroup 16384; longer rows are cut, and so are
+// rows too few to give the chip's CUs work, down to 2048 columns.
+int parts_of(int T, int V) {
+  if (V <= kRowCols) return 1;
+  const int least = (V + 16383) / 16384, most = (V + 2047) / 2048;
+  const int wanted = (512 + T - 1) / T;
+  return wanted < least ? least : wanted > most ? most : wanted;
+}
+int part_len(int T, int V) {
+  const int n = parts_of(T, V);
+  return ((V + n - 1) / n + 255) / 256 * 256;
+}
+
+template <class X, bool DIST, bool TOP>
+int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
+  const X* x = static_cast<const X*>(logits);
+  if (a.V <= kRowCols) {
+    a.nparts = 1;
+    a.part = kRowCols;
+    hipLaunchKernelGGL((rows_fwd_kernel<X, 1, kRowCols / 64, DIST, TOP>), dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
+    return check_launch("token_loss_rows");
+  }
+  a.part = part_len(a.T, a.V);
+  a.nparts = (a.V + a.part - 1) / a.part;
+  const int64_t grid = (int64_t)a.T * a.nparts;
+  RTE_REQUIRE(grid < ((int64_t)1 << 31), "token_loss: too many rows");
+  a.part_stats = static_cast<float4*>(ws);
+  a.part_keys = reinterpret_cast<u64*>(a.part_stats + grid);
+  auto fn = a.part <= 4096   ? rows_fwd_kernel<X, 4, 16, DIST, TOP>
+            : a.part <= 8192 ? rows_fwd_kernel<X, 4, 32, DIST, TOP>
+                             : rows_fwd_kernel<X, 4, 64, DIST, TOP>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  RTE_TRY(check_launch("token_loss_rows"));
+  if (a.nparts == 1) return 0;
+  hipLaunchKernelGGL((rows_join_kernel<X, DIST, TOP>), dim3(a.T), dim3(TOP ? 256 : 64), 0, s, x, a);
+  return check_launch("token_loss_join");
+}
+
+size_t rows_workspace(int T, int V, int n_top) {
+  if (T <= 0 || V <= kRowCols) return 0;
+  const int part = part_len(T, V), n = (V + part - 1) / part;
+  return n > 1 ? (size_t)T * n * (sizeof(float4) + n_top * sizeof(u64)) : 0;
+}
+
+bool fits_grid(int T, int V) { return (int64_t)T * ((V + kSeg - 1) / kSeg) < ((int64_t)1 << 31); }
 
 }  // namespace
 }  // namespace rte
@@ -250,7 +729,7 @@ using namespace rte;
 
 extern "C" {
 
-size_t rte_token_logprobs_workspace_bytes(int T, int V, int n_top) { return 0; }
+size_t rte_token_logprobs_workspace_bytes(int T, int V, int n_top) { return rows_workspace(T, V, n_top); }
 
 int rte_token_logprobs_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int64_t* tokens, float temperature,
                            int n_top, float* logprob, float* entropy, float* top_logprobs, int32_t* top_ids, float* stats,
@@ -261,14 +740,17 @@ int rte_token_logprobs_fwd(const void* logits, int64_t ld, int f32, int T, int V
   if (T == 0) return 0;
   RTE_REQUIRE(logits && tokens && logprob && entropy && (!n_top || (top_logprobs && top_ids)),
               "token_logprobs: null argument");
+  RTE_REQUIRE(fits_grid(T, V), "token_logprobs: too many rows");
+  const size_t need = rows_workspace(T, V, n_top);
+  RTE_REQUIRE(ws_bytes >= need && (ws || !need), "token_logprobs: workspace too small");
+  RowArgs a{};
+  a.ld = ld, a.T = T, a.V = V;
+  a.inv_t = 1.0f / temperature, a.c2 = (float)(1.4426950408889634 / temperature);
+  a.tokens = tokens, a.n_top = n_top, a.logprob = logprob, a.entropy = entropy, a.top_lp = top_logprobs;
+  a.top_ids = top_ids, a.stats = stats;
   auto s = static_cast<hipStream_t>(stream);
-  if (f32)
-    hipLaunchKernelGGL(logprobs_fwd_kernel<float>, dim3(T), dim3(kThreads), 0, s, static_cast<const float*>(logits), ld,
-                       V, tokens, 1.0f / temperature, n_top, logprob, entropy, top_logprobs, top_ids, stats);
-  else
-    hipLaunchKernelGGL(logprobs_fwd_kernel<bf16>, dim3(T), dim3(kThreads), 0, s, static_cast<const bf16*>(logits), ld, V,
-                       tokens, 1.0f / temperature, n_top, logprob, entropy, top_logprobs, top_ids, stats);
-  return check_launch("token_logprobs_fwd");
+  if (f32) return n_top ? launch_rows<float, false, true>(logits, a, ws, s) : launch_rows<float, false, false>(logits, a, ws, s);
+  return n_top ? launch_rows<bf16, false, true>(logits, a, ws, s) : launch_rows<bf16, false, false>(logits, a, ws, s);
 }
 
 int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V, const int64_t* tokens, float temperature,
@@ -278,50 +760,64 @@ int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V
   RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "token_logprobs_bwd: temperature must be positive and finite");
   if (T == 0) return 0;
   RTE_REQUIRE(logits && tokens && stats && entropy && dlogits, "token_logprobs_bwd: null argument");
+  RTE_REQUIRE(fits_grid(T, V), "token_logprobs_bwd: too many rows");
   auto s = static_cast<hipStream_t>(stream);
+  const int nseg = (V + kSeg - 1) / kSeg;
+  const int64_t items = (int64_t)T * nseg;
+  const dim3 grid((unsigned)((items + 3) / 4));
   if (f32)
-    hipLaunchKernelGGL(logprobs_bwd_kernel<float>, dim3(T), dim3(kThreads), 0, s, static_cast<const float*>(logits), ld,
-                       V, tokens, 1.0f / temperature, stats, entropy, g_logprob, g_entropy, static_cast<float*>(dlogits));
+    hipLaunchKernelGGL(logprobs_bwd_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(logits), ld, items, V,
+                       nseg, tokens, 1.0f / temperature, stats, entropy, g_logprob, g_entropy, static_cast<float*>(dlogits));
   else
-    hipLaunchKernelGGL(logprobs_bwd_kernel<bf16>, dim3(T), dim3(kThreads), 0, s, static_cast<const bf16*>(logits), ld, V,
-                       tokens, 1.0f / temperature, stats, entropy, g_logprob, g_entropy, static_cast<bf16*>(dlogits));
+    hipLaunchKernelGGL(logprobs_bwd_kernel<bf16>, grid, dim3(256), 0, s, static_cast<const bf16*>(logits), ld, items, V,
+                       nseg, tokens, 1.0f / temperature, stats, entropy, g_logprob, g_entropy, static_cast<bf16*>(dlogits));
   return check_launch("token_logprobs_bwd");
 }
 
-size_t rte_topk_distill_workspace_bytes(int T, int V, int K) { return 0; }
+size_t rte_topk_distill_workspace_bytes(int T, int V, int K) {
+  (void)K;
+  return rows_workspace(T, V, 0);
+}
 
 int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
-                         const float* teacher, int K, float temperature, int tail, float* loss, float* stats, void* ws,
-                         size_t ws_bytes, void* stream) {
+                         const float* teacher, int K, float temperature, int tail, float* loss, float* stats,
+                         int32_t* cols, float* coef, void* ws, size_t ws_bytes, void* stream) {
   RTE_REQUIRE(T >= 0 && V >= 1 && ld >= 0, "topk_distill: bad sizes");
   RTE_REQUIRE(K >= 1 && K <= kMaxTop, "topk_distill: list length must be in [1, %d]", kMaxTop);
   RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "topk_distill: temperature must be positive and finite");
   if (T == 0) return 0;
-  RTE_REQUIRE(logits && ids && teacher && loss, "topk_distill: null argument");
+  RTE_REQUIRE(logits && ids && teacher && loss && (!stats || (cols && coef)), "topk_distill: null argument");
+  RTE_REQUIRE(fits_grid(T, V), "topk_distill: too many rows");
+  const size_t need = rows_workspace(T, V, 0);
+  RTE_REQUIRE(ws_bytes >= need && (ws || !need), "topk_distill: workspace too small");
+  RowArgs a{};
+  a.ld = ld, a.T = T, a.V = V;
+  a.inv_t = 1.0f / temperature, a.c2 = (float)(1.4426950408889634 / temperature);
+  a.ids = ids, a.tl = teacher, a.K = K, a.tail = tail, a.it = 1.0 / temperature;
+  a.t2 = (double)temperature * temperature, a.loss = loss, a.stats = stats, a.cols = cols, a.coef = coef;
   auto s = static_cast<hipStream_t>(stream);
-  if (f32)
-    hipLaunchKernelGGL(distill_fwd_kernel<float>, dim3(T), dim3(kThreads), 0, s, static_cast<const float*>(logits), ld, V,
-                       ids, teacher, K, temperature, tail, loss, stats);
-  else
-    hipLaunchKernelGGL(distill_fwd_kernel<bf16>, dim3(T), dim3(kThreads), 0, s, static_cast<const bf16*>(logits), ld, V,
-                       ids, teacher, K, temperature, tail, loss, stats);
-  return check_launch("topk_distill_fwd");
+  return f32 ? launch_rows<float, true, false>(logits, a, ws, s) : launch_rows<bf16, true, false>(logits, a, ws, s);
 }
 
-int rte_topk_distill_bwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
-                         const float* teacher, int K, float temperature, int tail, const float* stats, const float* g,
-                         void* dlogits, void* stream) {
+int rte_topk_distill_bwd(const void* logits, int64_t ld, int f32, int T, int V, int K, float temperature,
+                         const float* stats, const int32_t* cols, const float* coef, const float* g, void* dlogits,
+                         void* stream) {
   RTE_REQUIRE(T >= 0 && V >= 1 && ld >= 0 && K >= 1 && K <= kMaxTop, "topk_distill_bwd: bad sizes");
   RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "topk_distill_bwd: temperature must be positive and finite");
   if (T == 0) return 0;
-  RTE_REQUIRE(logits && ids && teacher && stats && g && dlogits, "topk_distill_bwd: null argument");
+  RTE_REQUIRE(logits && stats && cols && coef && g && dlogits, "topk_distill_bwd: null argument");
+  RTE_REQUIRE(fits_grid(T, V), "topk_distill_bwd: too many rows");
   auto s = static_cast<hipStream_t>(stream);
+  const int nseg = (V + kSeg - 1) / kSeg;
+  const int64_t items = (int64_t)T * nseg;
+  const dim3 grid((unsigned)((items + 3) / 4));
+  const float c2 = (float)(1.4426950408889634 / temperature);
   if (f32)
-    hipLaunchKernelGGL(distill_bwd_kernel<float>, dim3(T), dim3(kThreads), 0, s, static_cast<const float*>(logits), ld, V,
-                       ids, teacher, K, temperature, tail, stats, g, static_cast<float*>(dlogits));
+    hipLaunchKernelGGL(distill_bwd_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(logits), ld, items, V,
+                       nseg, K, c2, temperature, stats, cols, coef, g, static_cast<float*>(dlogits));
   else
-    hipLaunchKernelGGL(distill_bwd_kernel<bf16>, dim3(T), dim3(kThreads), 0, s, static_cast<const bf16*>(logits), ld, V,
-                       ids, teacher, K, temperature, tail, stats, g, static_cast<bf16*>(dlogits));
+    hipLaunchKernelGGL(distill_bwd_kernel<bf16>, grid, dim3(256), 0, s, static_cast<const bf16*>(logits), ld, items, V,
+                       nseg, K, c2, temperature, stats, cols, coef, g, static_cast<bf16*>(dlogits));
   return check_launch("topk_distill_bwd");
 }
 

@@ -1745,8 +1745,9 @@ class LMHeadLogprobsFn(torch.autograd.Function):
             for lo in range(0, T, LMHeadLogprobsFn.ROWS):
                 hi = min(T, lo + LMHeadLogprobsFn.ROWS)
                 logits = gemm(hb[lo:hi], wb, out_f32=True)
+                ws = _scratch(_lib.load().rte_token_logprobs_workspace_bytes(hi - lo, V, 0), dev)
                 call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0, ptr(lp[lo:]),
-                     ptr(ent[lo:]), None, None, ptr(stats[lo:]), None, 0, _s())
+                     ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), ws.numel(), _s())
         ctx.save_for_backward(hb, wb, tk, stats, ent)
         ctx.meta = (shape, hidden.dtype, w.dtype, temperature)
         ctx.set_materialize_grads(False)
@@ -1768,9 +1769,10 @@ class LMHeadLogprobsFn(torch.autograd.Function):
             for lo in range(0, T, LMHeadLogprobsFn.ROWS):
                 hi = min(T, lo + LMHeadLogprobsFn.ROWS)
                 logits = gemm(hb[lo:hi], wb, out_f32=True)
+                dl = torch.empty_like(logits)
                 call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
-                     ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(logits), _s())
-                dl = logits.to(BF16)
+                     ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(dl), _s())
+                dl = dl.to(BF16)
                 if V % 8:
                     dl = torch.nn.functional.pad(dl, (0, -V % 8))
                 gemm(dl, wp, b_t=True, out=dh[lo:hi])
@@ -1810,14 +1812,16 @@ class TopkDistillFn(torch.autograd.Function):
         tc = teacher.detach().reshape(T, K).contiguous().to(F32)
         loss = torch.empty((T,), dtype=F32, device=dev)
         need = ctx.needs_input_grad[0]
-        stats = torch.empty((T, 6), dtype=F32, device=dev) if need else None
+        stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
+        cols = torch.empty((T, K), dtype=torch.int32, device=dev) if need else None
+        coef = torch.empty((T, K), dtype=F32, device=dev) if need else None
         with _on_device(dev):
             ws = _scratch(_lib.load().rte_topk_distill_workspace_bytes(T, V, K), dev)
             call("rte_topk_distill_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), K, temperature,
-                 int(tail), ptr(loss), ptr(stats), ptr(ws), ws.numel(), _s())
+                 int(tail), ptr(loss), ptr(stats), ptr(cols), ptr(coef), ptr(ws), ws.numel(), _s())
         if need:
-            ctx.save_for_backward(lg, ic, tc, stats)
-            ctx.meta = (logits.shape, ld, temperature, tail)
+            ctx.save_for_backward(lg, stats, cols, coef)
+            ctx.meta = (logits.shape, ld, temperature)
         ctx.set_materialize_grads(False)
         return loss.view(lead)
 
@@ -1826,14 +1830,14 @@ class TopkDistillFn(torch.autograd.Function):
     def backward(ctx, g):
         if g is None:
             return (None,) * 5
-        lg, ic, tc, stats = ctx.saved_tensors
-        shape, ld, temperature, tail = ctx.meta
+        lg, stats, cols, coef = ctx.saved_tensors
+        shape, ld, temperature = ctx.meta
         T, V = lg.shape
         gc = _row_grad(g, T)
         dx = torch.empty((T, V), dtype=lg.dtype, device=lg.device)
         with _on_device(lg.device):
-            call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), ic.shape[1],
-                 temperature, int(tail), ptr(stats), ptr(gc), ptr(dx), _s())
+            call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, cols.shape[1], temperature,
+                 ptr(stats), ptr(cols), ptr(coef), ptr(gc), ptr(dx), _s())
         return dx.view(shape), None, None, None, None
 
 

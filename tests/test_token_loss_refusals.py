@@ -26,6 +26,8 @@ def test_token_logprobs(lib):
 
     fwd(T=-1), fwd(V=0), fwd(ld=-1), fwd(n=-1), fwd(n=129, V=1000), fwd(n=65), fwd(t=0.0), fwd(t=float("nan"))
     fwd(t=float("inf")), fwd(x=None), fwd(tok=None), fwd(lp=None), fwd(ent=None), fwd(tl=None), fwd(ti=None)
+    fwd(V=100000, wsn=lib.rte_token_logprobs_workspace_bytes(4, 100000, 8) - 1), fwd(V=100000, ws=None)
+    fwd(T=(1 << 31) - 1, V=1 << 20)
     for a in ((None, 64, 1, 4, 64, BUF, 1.0, BUF, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, 1.0, None, BUF, BUF, BUF, BUF),
               (BUF, 64, 1, 4, 64, BUF, -1.0, BUF, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 0, BUF, 1.0, BUF, BUF, BUF, BUF, BUF),
               (BUF, 64, 1, 4, 64, BUF, 1.0, BUF, BUF, BUF, BUF, None)):
@@ -35,15 +37,18 @@ def test_token_logprobs(lib):
 
 
 def test_topk_distill(lib):
-    def fwd(x=BUF, ld=64, T=4, V=64, ids=BUF, tl=BUF, K=8, t=1.0, loss=BUF, ws=BUF, wsn=1 << 40):
-        refused(lib, "rte_topk_distill_fwd", x, ld, 1, T, V, ids, tl, K, t, 0, loss, BUF, ws, wsn, None)
+    def fwd(x=BUF, ld=64, T=4, V=64, ids=BUF, tl=BUF, K=8, t=1.0, loss=BUF, cols=BUF, coef=BUF, ws=BUF,
+            wsn=1 << 40):
+        refused(lib, "rte_topk_distill_fwd", x, ld, 1, T, V, ids, tl, K, t, 0, loss, BUF, cols, coef, ws, wsn, None)
 
     fwd(T=-1), fwd(V=0), fwd(ld=-1), fwd(K=0), fwd(K=129), fwd(t=0.0), fwd(t=float("nan")), fwd(t=float("inf"))
-    fwd(x=None), fwd(ids=None), fwd(tl=None), fwd(loss=None)
-    for a in ((BUF, 64, 1, 4, 64, BUF, BUF, 0, 1.0, 0, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, BUF, 8, 0.0, 0, BUF, BUF, BUF),
-              (BUF, 64, 1, 4, 64, BUF, BUF, 8, 1.0, 0, None, BUF, BUF), (BUF, 64, 1, 4, 64, BUF, BUF, 8, 1.0, 0, BUF, None, BUF)):
+    fwd(x=None), fwd(ids=None), fwd(tl=None), fwd(loss=None), fwd(cols=None), fwd(coef=None)
+    fwd(V=100000, wsn=lib.rte_topk_distill_workspace_bytes(4, 100000, 8) - 1), fwd(V=100000, ws=None)
+    fwd(T=(1 << 31) - 1, V=1 << 20)
+    for a in ((BUF, 64, 1, 4, 64, 0, 1.0, BUF, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, 8, 0.0, BUF, BUF, BUF, BUF, BUF),
+              (BUF, 64, 1, 4, 64, 8, 1.0, None, BUF, BUF, BUF, BUF), (BUF, 64, 1, 4, 64, 8, 1.0, BUF, BUF, BUF, None, BUF)):
         refused(lib, "rte_topk_distill_bwd", *a, None)
-    assert lib.rte_topk_distill_fwd(None, 64, 1, 0, 64, None, None, 8, 1.0, 0, None, None, None, 0, None) == 0
+    assert lib.rte_topk_distill_fwd(None, 64, 1, 0, 64, None, None, 8, 1.0, 0, None, None, None, None, None, 0, None) == 0
 
 
 def test_pool_balance(lib):
