@@ -13,79 +13,13 @@
 //   tail 1: p_j = e^{t_j}, r = 1 - sum p_j   L = t^2 (sum_j p_j (log p_j - log q_{c_j}) + r (log r - log q(R)))
 //   dx_v  = g t (q_v - p_j) where v = c_j, else g t (q_v - r q_v / q(R)) (tail 0: r = 0)
 #include "../../include/rte_hip.h"
-#include "common.hpp"
+#include "row_words.hpp"
 
 namespace rte {
 
 namespace {
 
 constexpr int kMaxTop = 128;  // alternatives or list entries per row
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-
-// Sixteen bytes of a row at any alignment of its element type: rows of odd length start anywhere, and a
-// global load or store of four words asks for no more.
-typedef uint32_t words_v __attribute__((ext_vector_type(4), aligned(2), may_alias));
-struct Words {
-  uint32_t w[4];
-};
-
-template <class X>
-struct Row;
-template <>
-struct Row<float> {
-  static constexpr int VE = 4;
-  __device__ static float one(const float* x, int64_t i) { return x[i]; }
-  __device__ static void put(float* x, int64_t i, float v) { x[i] = v; }
-  __device__ static float get(const Words& v, int j) { return __uint_as_float(v.w[j]); }
-  __device__ static void set(Words& v, int j, float f) { v.w[j] = __float_as_uint(f); }
-  __device__ static Words pack(const float* f) {
-    return {{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}};
-  }
-};
-template <>
-struct Row<bf16> {
-  static constexpr int VE = 8;
-  __device__ static float one(const bf16* x, int64_t i) { return bf2f(x[i]); }
-  __device__ static void put(bf16* x, int64_t i, float v) { x[i] = f2bf(v); }
-  __device__ static float get(const Words& v, int j) {
-    return __uint_as_float(j & 1 ? v.w[j >> 1] & 0xffff0000u : v.w[j >> 1] << 16);
-  }
-  __device__ static void set(Words& v, int j, float f) {
-    const uint32_t h = __float_as_uint(f) >> 16;
-    v.w[j >> 1] = j & 1 ? (v.w[j >> 1] & 0xffffu) | h << 16 : (v.w[j >> 1] & 0xffff0000u) | h;
-  }
-  __device__ static Words pack(const float* f) {
-    return {{pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7])}};
-  }
-};
-
-// Elements at .. at + VE of a row that ends at `end`; what lies past the end is -inf.
-template <class X>
-__device__ __forceinline__ Words load_words(const X* row, int at, int end) {
-  constexpr int VE = Row<X>::VE;
-  Words r;
-  if (at + VE <= end) {
-    const words_v v = *reinterpret_cast<const words_v*>(row + at);
-    r = {{v.x, v.y, v.z, v.w}};
-  } else {
-#pragma unroll
-    for (int j = 0; j < VE; ++j) Row<X>::set(r, j, at + j < end ? Row<X>::one(row, at + j) : -INFINITY);
-  }
-  return r;
-}
-
-template <class X>
-__device__ __forceinline__ void store_words(X* row, int at, int end, const float* f) {
-  constexpr int VE = Row<X>::VE;
-  if (at + VE <= end) {
-    const Words p = Row<X>::pack(f);
-    *reinterpret_cast<words_v*>(row + at) = words_v{p.w[0], p.w[1], p.w[2], p.w[3]};
-  } else {
-#pragma unroll
-    for (int j = 0; j < VE; ++j)
-      if (at + j < end) Row<X>::put(row, at + j, f[j]);
-  }
-}
 
 // Order of the alternatives as unsigned keys: larger value first, -0 = +0, NaN above everything.
 constexpr uint32_t kNanKey = 0xfffffffeu, kInfKey = 0xff800000u;
@@ -98,24 +32,6 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k > kInfKey ? 0x7fc00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 __device__ __forceinline__ u64 full_key(float x, int col) { return (u64)value_key(x) << 32 | (uint32_t)~col; }
-
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-
-template <class V>
-__device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-template <class V>
-__device__ __forceinline__ V wave_max(V v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const V u = __shfl_xor(v, o, 64);
-    v = u > v || v != v ? u : v;  // NaN loses
-  }
-  return v;
-}
 
 struct RowArgs {
   int64_t ld;

@@ -56,6 +56,7 @@ def check(H, x, ids, mask=None, gb=0.7, gz=0.3):
     bal, z, counts = H.pool_balance(leaf, ids, mask=mask)
     (dx,) = torch.autograd.grad((bal, z), leaf, (torch.tensor(gb, device=DEV), torch.tensor(gz, device=DEV)))
     torch.cuda.synchronize()
+    bal, z = bal.detach(), z.detach()
     wb, wz, wc, wd, scale, lse = want64(x.detach(), ids.long(), mask, gb, gz)
     assert counts.dtype == torch.int32 and torch.equal(counts.long(), wc)
     fin = torch.isfinite(x.detach())

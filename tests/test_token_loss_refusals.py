@@ -58,6 +58,7 @@ def test_pool_balance(lib):
     def fwd(x=BUF, ld=64, T=1000, C=64, ids=BUF, k=8, out=BUF, cnt=BUF, frac=BUF, ws=BUF, wsn=need):
         refused(lib, "rte_pool_balance_fwd", x, ld, 1, T, C, ids, k, None, out, cnt, frac, ws, wsn, None)
 
+    fwd(T=1 << 28, k=8, wsn=1 << 40)
     fwd(T=-1), fwd(C=0), fwd(C=1025), fwd(k=0), fwd(ld=-1), fwd(x=None), fwd(ids=None), fwd(out=None), fwd(cnt=None)
     fwd(frac=None), fwd(ws=None), fwd(wsn=need - 1)
     refused(lib, "rte_pool_balance_bwd", BUF, 64, 1, 4, 1025, None, BUF, None, None, BUF, None)
