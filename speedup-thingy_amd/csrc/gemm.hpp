@@ -41,6 +41,8 @@ enum EpiKind : int {
   EPI_SWIGLU_FWD = 1,   // columns interleaved per 64: [32 up | 32 gate]; writes UG and Z
   EPI_SWIGLU_BWD = 2,   // acc = dZ; reads UG; writes dUG (+ optional per-row <z, acc>)
   EPI_ROPE_QKV = 3,     // columns [q | k | v]; interleaved RoPE on q,k; writes [B,H,S,hd]
+  EPI_ROW_SUMS = 4,     // acc = logits, not stored; softmax sums of every 64 columns and the token's logit
+  EPI_DLOGITS = 5,      // acc = logits, not stored; C (bf16) = their gradient for log probability and entropy
 };
 
 enum GemmMode : int { MODE_DENSE = 0, MODE_GROUP_M = 1, MODE_GROUP_K = 2 };
@@ -74,6 +76,14 @@ struct Epilogue {
   const float* cos_t = nullptr;      // [S, hd]
   const float* sin_t = nullptr;
   int S = 0, H = 0, hd = 0, dmodel = 0;
+  // log probabilities: columns are tokens of the vocabulary, col0 first
+  float c2 = 0.0f, inv_t = 0.0f;     // log2(e) / temperature, 1 / temperature
+  int col0 = 0;
+  const int64_t* tokens = nullptr;   // [M]
+  float4* row_part = nullptr;        // fwd: [ceil(N / 64), M] {max, sum, sum of e u, -}
+  float* tok_logit = nullptr;        // fwd: [M], written where the token is one of the columns
+  const float4* row_in = nullptr;    // bwd: [M] {max, log sum, g + g_H entropy, g_H}
+  const float* g_tok = nullptr;      // bwd: [M] g (0: no token)
 };
 
 struct GemmArgs {

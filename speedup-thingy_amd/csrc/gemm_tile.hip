@@ -15,6 +15,7 @@
 // of products to arrive.
 #include "gemm_dev.hpp"
 #include "gemm_tile.hpp"
+#include "row_words.hpp"
 
 #include <type_traits>
 
@@ -159,6 +160,54 @@ __device__ __forceinline__ float swiglu_bwd8(const Epilogue& e, int m, int n, co
   *reinterpret_cast<uint4*>(e.ug + at) = make_uint4(du[0], du[1], du[2], du[3]);
   *reinterpret_cast<uint4*>(e.ug + at + 32) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
   return part;
+}
+
+// Softmax sums of row m's logits n .. n + 7 with those of the seven other lanes of its 64-column block, and the
+// token's logit where it is one of them.  (Rows past the end are computed and not stored.)
+__device__ __forceinline__ void row_sums8(const Epilogue& e, int m, int mlim, int n, int N, int M, const float* at,
+                                          int lane) {
+  const float4 x = *reinterpret_cast<const float4*>(at);
+  const float4 y = *reinterpret_cast<const float4*>(at + 4);
+  float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  if (n + 8 > N) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = n + t < N ? v[t] : -INFINITY;
+  }
+  float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  mx = wave_max<8>(mx);
+  const float m0 = mx == -INFINITY ? 0.0f : mx;
+  float s = 0.0f, su = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const float u = (v[t] - m0) * e.c2, w = exp2_(u);
+    s += w;
+    su += w * fmaxf(u, -256.0f);
+  }
+  s = wave_sum<8>(s);
+  su = wave_sum<8>(su);
+  if (m >= mlim) return;
+  if ((lane & 7) == 0 && n < N) e.row_part[(int64_t)(n >> 6) * M + m] = make_float4(mx, s, su, 0.0f);
+  const int64_t rel = e.tokens[m] - n;
+  if (rel >= 0 && rel < 8 && n + rel < N) e.tok_logit[m] = at[rel];
+}
+
+// Gradient of row m's logits n .. n + 7: ([column = token] g - p (g + g_H (log p + entropy))) / temperature.
+__device__ __forceinline__ void dlogits8(const Epilogue& e, int m, int n, const float* at) {
+  const float4 x = *reinterpret_cast<const float4*>(at);
+  const float4 y = *reinterpret_cast<const float4*>(at + 4);
+  const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  const float4 r = e.row_in[m];
+  const float g = e.g_tok[m];
+  const int64_t rel = g != 0.0f ? e.tokens[m] - e.col0 - n : -1;
+  float d[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const float lp = (v[t] - r.x) * e.inv_t - r.y;
+    d[t] = ((t == rel ? g : 0.0f) - exp2_(lp * kLog2e) * (r.z + r.w * fmaxf(lp, -200.0f))) * e.inv_t;
+  }
+  bf16* out = static_cast<bf16*>(e.c) + (int64_t)m * e.ldc + n;
+  *reinterpret_cast<uint4*>(out) =
+      make_uint4(pack_bf2(d[0], d[1]), pack_bf2(d[2], d[3]), pack_bf2(d[4], d[5]), pack_bf2(d[6], d[7]));
 }
 
 template <int BM, int BN, int WM, int WN, int BK, int ST, bool AT, bool BT, int EPI, int MODE>
@@ -511,7 +560,15 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
             if (e.dw_row && m < mlim && (lane & 7) == 0) e.dw_row[m] = part;
             continue;
           }
+          if constexpr (EPI == EPI_ROW_SUMS) {
+            row_sums8(e, m, mlim, n, p.N, p.M, pt + row * kPatchPitch + cc, lane);
+            continue;
+          }
           if (m >= mlim || n >= p.N) continue;
+          if constexpr (EPI == EPI_DLOGITS) {
+            dlogits8(e, m, n, pt + row * kPatchPitch + cc);
+            continue;
+          }
           if constexpr (EPI == EPI_SWIGLU_BWD && MODE != MODE_GROUP_M) {
             swiglu_bwd8(e, m, n, pt + row * kPatchPitch + cc);
             continue;
@@ -794,6 +851,8 @@ int gemm_tile_launch(const GemmArgs& p0, int epi_kind, hipStream_t stream, int v
     case EPI_STORE: return launch_tile<EPI_STORE>(p, stream, vec, tile);
     case EPI_SWIGLU_FWD: return launch_tile<EPI_SWIGLU_FWD>(p, stream, vec, tile);
     case EPI_SWIGLU_BWD: return launch_tile<EPI_SWIGLU_BWD>(p, stream, vec, tile);
+    case EPI_ROW_SUMS: return launch_tile<EPI_ROW_SUMS>(p, stream, vec, tile);
+    case EPI_DLOGITS: return launch_tile<EPI_DLOGITS>(p, stream, vec, tile);
     default: return launch_tile<EPI_ROPE_QKV>(p, stream, vec, tile);
   }
 }

@@ -1656,6 +1656,11 @@ def _check_logits(op: str, logits: torch.Tensor) -> None:
         raise ValueError(f"{op}: unsupported logits {tuple(logits.shape)}")
 
 
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    """t, copied where it starts inside a 16-byte word."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _row_grad(g, T: int):
     return None if g is None else g.reshape(T).contiguous().to(F32)
 
@@ -1725,29 +1730,40 @@ def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
 
 
 class LMHeadLogprobsFn(torch.autograd.Function):
-    """token_logprobs' first two results of hidden @ W^T without keeping the logits: the backward computes
-    them again, a range of tokens at a time."""
+    """token_logprobs' first two results of hidden @ W^T without keeping the logits.
+
+    Where the tile product takes the sizes (rte_lm_head_logprobs_ok) the logits stay in its accumulators;
+    the backward multiplies again, GRAD bytes of logit gradients at a time.  Other widths go through
+    fp32 logits of ROWS tokens at a time."""
 
     ROWS = 2048
+    GRAD = 1 << 30
 
     @staticmethod
     def forward(ctx, hidden, w, tokens, temperature: float):
         shape = hidden.shape
-        hb = hidden.reshape(-1, shape[-1]).contiguous().to(BF16)
-        wb = cast_bf16(w)
-        T, V = hb.shape[0], wb.shape[0]
+        hb = _aligned16(hidden.reshape(-1, shape[-1]).contiguous().to(BF16))
+        wb = _aligned16(cast_bf16(w))
+        T, d = hb.shape
+        V = wb.shape[0]
         dev = hb.device
+        lib = _lib.load()
         tk = tokens.reshape(T).contiguous().to(torch.int64)
         lp = torch.empty((T,), dtype=F32, device=dev)
         ent = torch.empty((T,), dtype=F32, device=dev)
         stats = torch.empty((T, 2), dtype=F32, device=dev)
         with _on_device(dev):
-            for lo in range(0, T, LMHeadLogprobsFn.ROWS):
-                hi = min(T, lo + LMHeadLogprobsFn.ROWS)
-                logits = gemm(hb[lo:hi], wb, out_f32=True)
-                ws = _scratch(_lib.load().rte_token_logprobs_workspace_bytes(hi - lo, V, 0), dev)
-                call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0, ptr(lp[lo:]),
-                     ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), ws.numel(), _s())
+            if lib.rte_lm_head_logprobs_ok(T, d, V):
+                ws = _scratch(lib.rte_lm_head_logprobs_workspace_bytes(T, V), dev)
+                call("rte_lm_head_logprobs_fwd", ptr(hb), ptr(wb), T, d, V, ptr(tk), temperature, ptr(lp), ptr(ent),
+                     ptr(stats), ptr(ws), ws.numel(), _s())
+            else:
+                for lo in range(0, T, LMHeadLogprobsFn.ROWS):
+                    hi = min(T, lo + LMHeadLogprobsFn.ROWS)
+                    logits = gemm(hb[lo:hi], wb, out_f32=True)
+                    ws = _scratch(lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0), dev)
+                    call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0,
+                         ptr(lp[lo:]), ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), ws.numel(), _s())
         ctx.save_for_backward(hb, wb, tk, stats, ent)
         ctx.meta = (shape, hidden.dtype, w.dtype, temperature)
         ctx.set_materialize_grads(False)
@@ -1761,23 +1777,64 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         hb, wb, tk, stats, ent = ctx.saved_tensors
         shape, h_dt, w_dt, temperature = ctx.meta
         T, V = hb.shape[0], wb.shape[0]
+        need_h, need_w = ctx.needs_input_grad[:2]
         gl, ge = _row_grad(g_lp, T), _row_grad(g_ent, T)
+        if T == 0:
+            dh, dw = hb.new_zeros(hb.shape), wb.new_zeros(wb.shape)
+        else:
+            fused = V % 8 == 0 and _lib.load().rte_lm_head_logprobs_ok(T, hb.shape[1], V)
+            grads = LMHeadLogprobsFn._grads if fused else LMHeadLogprobsFn._grads_by_rows
+            with _on_device(hb.device):
+                dh, dw = grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_dt == BF16)
+        return dh.view(shape).to(h_dt) if need_h else None, dw.to(w_dt) if need_w else None, None, None
+
+    @staticmethod
+    def _grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_bf16):
+        """Vocabulary range by vocabulary range: the gradient of its logits in bf16, then dW's rows of that
+        range and the range's part of dh (fp32 until the last).  Whole 64s of columns first: the tile product
+        of dh takes those."""
+        lib = _lib.load()
+        T, d = hb.shape
+        V = wb.shape[0]
+        dev = hb.device
+        width = max(64, LMHeadLogprobsFn.GRAD // (2 * T) // 64 * 64)
+        whole = V // 64 * 64
+        cuts = [*range(0, whole, width), whole] if whole else [0]
+        if whole < V:
+            cuts.append(V)
+        dh = torch.empty((T, d), dtype=BF16 if len(cuts) == 2 else F32, device=dev) if need_h else None
+        dw = torch.empty((V, d), dtype=BF16 if w_bf16 else F32, device=dev) if need_w else None
+        ws = _scratch(lib.rte_lm_head_dlogits_workspace_bytes(T), dev)
+        for lo, hi in zip(cuts, cuts[1:]):
+            dl = torch.empty((T, hi - lo), dtype=BF16, device=dev)
+            call("rte_lm_head_dlogits", ptr(hb), ptr(wb), T, d, V, lo, hi - lo, ptr(tk), temperature, ptr(stats), ptr(ent),
+                 ptr(gl), ptr(ge), ptr(dl), ptr(ws), ws.numel(), _s())
+            if need_h:
+                gemm(dl, wb[lo:hi], b_t=True, out=dh, beta=float(lo > 0))
+            if need_w:
+                gemm(dl, hb, a_t=True, b_t=True, out=dw[lo:hi])
+        return dh, dw
+
+    @staticmethod
+    def _grads_by_rows(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_bf16):
+        T, V = hb.shape[0], wb.shape[0]
         dh = torch.empty_like(hb)
         dw = torch.zeros(wb.shape, dtype=F32, device=hb.device)
         wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
-        with _on_device(hb.device):
-            for lo in range(0, T, LMHeadLogprobsFn.ROWS):
-                hi = min(T, lo + LMHeadLogprobsFn.ROWS)
-                logits = gemm(hb[lo:hi], wb, out_f32=True)
-                dl = torch.empty_like(logits)
-                call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
-                     ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(dl), _s())
-                dl = dl.to(BF16)
-                if V % 8:
-                    dl = torch.nn.functional.pad(dl, (0, -V % 8))
+        for lo in range(0, T, LMHeadLogprobsFn.ROWS):
+            hi = min(T, lo + LMHeadLogprobsFn.ROWS)
+            logits = gemm(hb[lo:hi], wb, out_f32=True)
+            dl = torch.empty_like(logits)
+            call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
+                 ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(dl), _s())
+            dl = dl.to(BF16)
+            if V % 8:
+                dl = torch.nn.functional.pad(dl, (0, -V % 8))
+            if need_h:
                 gemm(dl, wp, b_t=True, out=dh[lo:hi])
+            if need_w:
                 dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True)[:V]
-        return dh.view(shape).to(h_dt), dw.to(w_dt), None, None
+        return dh, dw
 
 
 def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:

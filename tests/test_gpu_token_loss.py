@@ -289,7 +289,7 @@ def head64(h, w, tok, t, g_lp, g_h):
 
 
 @pytest.mark.parametrize("T,d,V", [(1, 8, 1), (1, 64, 300), (3, 64, 17), (65, 72, 129), (64, 128, 256), (200, 512, 2048),
-                                   (129, 256, 1000), (300, 128, 8200), (257, 64, 515), (33, 1024, 4099), (2100, 64, 640),
+                                   (129, 256, 1000), (300, 128, 8200), (257, 64, 515), (33, 1024, 4099), (2100, 64, 640), (1, 128, 1), (2, 128, 8), (255, 192, 24), (257, 128, 72), (600, 256, 3000),
                                    (512, 512, 512)])
 @pytest.mark.parametrize("t", [1.0, 0.7])
 def test_head_sizes(H, T, d, V, t):
@@ -344,6 +344,37 @@ def test_head_forms(H):
     lp, _ = H.lm_head_logprobs(h, w, torch.full_like(tok, -1))
     dh, dw = torch.autograd.grad(lp, (h, w), up)
     assert not lp.any() and not dh.any() and not dw.any()
+
+
+@pytest.mark.parametrize("V", [640, 1096, 2056])
+def test_head_by_vocabulary_ranges(H, V, monkeypatch):
+    """A small budget of logit gradients: several ranges, the last of them less than 64 columns."""
+    g = gen(V, 18)
+    T, d = 100, 192
+    h = torch.randn(T, d, device=DEV, generator=g).bfloat16().requires_grad_()
+    w = (torch.randn(V, d, device=DEV, generator=g) * 0.2).bfloat16().requires_grad_()
+    tok = torch.randint(0, V, (T,), device=DEV, generator=g)
+    up = torch.randn(T, device=DEV, generator=g)
+    monkeypatch.setattr(H.LMHeadLogprobsFn, "GRAD", 2 * T * 300)
+    lp, ent = H.lm_head_logprobs(h, w, tok)
+    dh, dw = torch.autograd.grad((lp, ent), (h, w), (up, up))
+    out, e, xh, xw, sh, sw, za, zmax = head64(h, w, tok, 1.0, up, up)
+    c = ulps(V, 2 * zmax) + 2 * d * 2.0 ** -24 * za
+    rel = 2.0 ** -8 + 4 * c + 2.0 ** -20
+    near(lp, out, c + 2.0 ** -22 * out.abs(), "logprob")
+    near(dh, xh, rel * sh + 2.0 ** -8 * xh.abs() + 1e-37, "hidden gradient")
+    near(dw, xw, rel * sw + 2.0 ** -8 * xw.abs() + 1e-37, "weight gradient")
+
+
+def test_head_off_alignment(H):
+    """Hidden states and a matrix that start two bytes into a word."""
+    g = gen(19)
+    T, d, V = 70, 128, 320
+    h = torch.randn(T * d + 1, device=DEV, generator=g).bfloat16()[1:].view(T, d)
+    w = (torch.randn(V * d + 1, device=DEV, generator=g) * 0.2).bfloat16()[1:].view(V, d)
+    tok = torch.randint(0, V, (T,), device=DEV, generator=g)
+    a, b = H.lm_head_logprobs(h, w, tok), H.lm_head_logprobs(h.clone(), w.clone(), tok)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
 def test_head_agrees_with_the_stored_logits(H):

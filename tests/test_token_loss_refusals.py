@@ -36,6 +36,26 @@ def test_token_logprobs(lib):
     assert lib.rte_token_logprobs_bwd(None, 64, 1, 0, 64, None, 1.0, None, None, None, None, None, None) == 0
 
 
+def test_lm_head_logprobs(lib):
+    ok = lib.rte_lm_head_logprobs_ok
+    assert ok(1, 128, 1) and ok(8192, 1024, 32768)
+    assert not any(ok(*a) for a in ((0, 128, 10), (10, 128, 0), (10, 64, 10), (10, 160, 10), (1 << 23, 128, 10), (10, 128, 1 << 23)))
+    need = lib.rte_lm_head_logprobs_workspace_bytes(100, 1000)
+
+    def fwd(h=BUF, w=BUF, T=100, d=128, V=1000, tok=BUF, t=1.0, lp=BUF, ent=BUF, st=BUF, ws=BUF, wsn=need):
+        refused(lib, "rte_lm_head_logprobs_fwd", h, w, T, d, V, tok, t, lp, ent, st, ws, wsn, None)
+
+    fwd(d=100), fwd(T=0), fwd(V=0), fwd(t=0.0), fwd(t=float("nan")), fwd(h=None), fwd(w=None), fwd(tok=None), fwd(lp=None)
+    fwd(ent=None), fwd(st=None), fwd(ws=None), fwd(wsn=need - 1), fwd(h=BUF + 2), fwd(w=BUF + 8)
+    room = lib.rte_lm_head_dlogits_workspace_bytes(100)
+
+    def bwd(h=BUF, w=BUF, T=100, d=128, V=1000, c=0, n=64, tok=BUF, t=1.0, st=BUF, ent=BUF, dl=BUF, ws=BUF, wsn=room):
+        refused(lib, "rte_lm_head_dlogits", h, w, T, d, V, c, n, tok, t, st, ent, BUF, BUF, dl, ws, wsn, None)
+
+    bwd(c=-8), bwd(c=944), bwd(n=0), bwd(n=60), bwd(n=1008), bwd(d=100), bwd(t=-1.0), bwd(st=None), bwd(ent=None)
+    bwd(dl=None), bwd(dl=BUF + 4), bwd(ws=None), bwd(wsn=room - 1), bwd(tok=None), bwd(h=None), bwd(w=None)
+
+
 def test_topk_distill(lib):
     def fwd(x=BUF, ld=64, T=4, V=64, ids=BUF, tl=BUF, K=8, t=1.0, loss=BUF, cols=BUF, coef=BUF, ws=BUF,
             wsn=1 << 40):
