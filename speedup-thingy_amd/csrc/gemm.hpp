@@ -41,8 +41,8 @@ enum EpiKind : int {
   EPI_SWIGLU_FWD = 1,   // columns interleaved per 64: [32 up | 32 gate]; writes UG and Z
   EPI_SWIGLU_BWD = 2,   // acc = dZ; reads UG; writes dUG (+ optional per-row <z, acc>)
   EPI_ROPE_QKV = 3,     // columns [q | k | v]; interleaved RoPE on q,k; writes [B,H,S,hd]
-  EPI_ROW_SUMS = 4,     // acc = logits, not stored; softmax sums of every 64 columns and the token's logit
-  EPI_DLOGITS = 5,      // acc = logits, not stored; C (bf16) = their gradient for log probability and entropy
+  EPI_ROW_SUMS = 4,     // acc = logits^T, not stored; softmax sums of a wave's block, the token's logit
+  EPI_DLOGITS = 5,      // acc = logits^T, not stored; C[n, m] (bf16) = the logits' gradient
 };
 
 enum GemmMode : int { MODE_DENSE = 0, MODE_GROUP_M = 1, MODE_GROUP_K = 2 };
@@ -76,14 +76,13 @@ struct Epilogue {
   const float* cos_t = nullptr;      // [S, hd]
   const float* sin_t = nullptr;
   int S = 0, H = 0, hd = 0, dmodel = 0;
-  // log probabilities: columns are tokens of the vocabulary, col0 first
-  float c2 = 0.0f, inv_t = 0.0f;     // log2(e) / temperature, 1 / temperature
+  // log probabilities: the product is taken as w h^T, m counts the vocabulary (col0 first), n the rows of h
+  float c2 = 0.0f;                   // log2(e) / temperature
   int col0 = 0;
-  const int64_t* tokens = nullptr;   // [M]
-  float4* row_part = nullptr;        // fwd: [ceil(N / 64), M] {max, sum, sum of e u, -}
-  float* tok_logit = nullptr;        // fwd: [M], written where the token is one of the columns
-  const float4* row_in = nullptr;    // bwd: [M] {max, log sum, g + g_H entropy, g_H}
-  const float* g_tok = nullptr;      // bwd: [M] g (0: no token)
+  const int64_t* tokens = nullptr;   // [N]
+  float4* row_part = nullptr;        // EPI_ROW_SUMS: [gemm_tile_row_blocks, N] {max, sum 2^u, sum 2^u u, -}, u in log2
+  float* tok_logit = nullptr;        // EPI_ROW_SUMS: [N], written where the token is one of the columns
+  const float4* row_in = nullptr;    // EPI_DLOGITS: [N] {log2 of the normaliser, a, b, g / t}: d = 2^lp (a + b lp)
 };
 
 struct GemmArgs {

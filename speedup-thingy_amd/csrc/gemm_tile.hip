@@ -162,52 +162,97 @@ __device__ __forceinline__ float swiglu_bwd8(const Epilogue& e, int m, int n, co
   return part;
 }
 
-// Softmax sums of row m's logits n .. n + 7 with those of the seven other lanes of its 64-column block, and the
-// token's logit where it is one of them.  (Rows past the end are computed and not stored.)
-__device__ __forceinline__ void row_sums8(const Epilogue& e, int m, int mlim, int n, int N, int M, const float* at,
-                                          int lane) {
-  const float4 x = *reinterpret_cast<const float4*>(at);
-  const float4 y = *reinterpret_cast<const float4*>(at + 4);
-  float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-  if (n + 8 > N) {
+// Log probabilities.  The product is w h^T, so a lane's accumulators hold logits of one row of h (column l32 of a
+// 32 x 32 block), rows 8 q + 4 half + 0 .. 3 of the vocabulary: a row's sums need no exchange but between the
+// two halves of the wave.  (As h w^T, through 64-column patches in LDS and three exchanges per sum, the
+// epilogue took 11 us of a 256 x 256 tile's 39; this one see the launch.)
+template <int J, int I0, int TM, int TMA, int TN>
+__device__ __forceinline__ float find_logit(const f32x16_v (&acc)[TMA][TN], int rel, int half) {
+  float x = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) v[t] = n + t < N ? v[t] : -INFINITY;
-  }
-  float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
-  mx = wave_max<8>(mx);
-  const float m0 = mx == -INFINITY ? 0.0f : mx;
-  float s = 0.0f, su = 0.0f;
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const float u = (v[t] - m0) * e.c2, w = exp2_(u);
-    s += w;
-    su += w * fmaxf(u, -256.0f);
-  }
-  s = wave_sum<8>(s);
-  su = wave_sum<8>(su);
-  if (m >= mlim) return;
-  if ((lane & 7) == 0 && n < N) e.row_part[(int64_t)(n >> 6) * M + m] = make_float4(mx, s, su, 0.0f);
-  const int64_t rel = e.tokens[m] - n;
-  if (rel >= 0 && rel < 8 && n + rel < N) e.tok_logit[m] = at[rel];
+    for (int r = 0; r < 16; ++r) x = rel == i * 32 + 8 * (r >> 2) + 4 * half + (r & 3) ? acc[I0 + i][J][r] : x;
+  return x;
 }
 
-// Gradient of row m's logits n .. n + 7: ([column = token] g - p (g + g_H (log p + entropy))) / temperature.
-__device__ __forceinline__ void dlogits8(const Epilogue& e, int m, int n, const float* at) {
-  const float4 x = *reinterpret_cast<const float4*>(at);
-  const float4 y = *reinterpret_cast<const float4*>(at + 4);
-  const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-  const float4 r = e.row_in[m];
-  const float g = e.g_tok[m];
-  const int64_t rel = g != 0.0f ? e.tokens[m] - e.col0 - n : -1;
-  float d[8];
+// Sums of the wave's WTM vocabulary rows from m0 on for row n of h; left = vocabulary rows that exist from m0.
+template <int J, int TM, int TN>
+__device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][TN], int m0, int left, int n, int N, int half) {
+  if (left < TM * 32) {
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const float lp = (v[t] - r.x) * e.inv_t - r.y;
-    d[t] = ((t == rel ? g : 0.0f) - exp2_(lp * kLog2e) * (r.z + r.w * fmaxf(lp, -200.0f))) * e.inv_t;
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (i * 32 + 8 * (r >> 2) + 4 * half + (r & 3) >= left) acc[i][J][r] = -INFINITY;
   }
-  bf16* out = static_cast<bf16*>(e.c) + (int64_t)m * e.ldc + n;
-  *reinterpret_cast<uint4*>(out) =
-      make_uint4(pack_bf2(d[0], d[1]), pack_bf2(d[2], d[3]), pack_bf2(d[4], d[5]), pack_bf2(d[6], d[7]));
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) mx = fmaxf(mx, fmaxf(acc[i][J][r], acc[i][J][r + 1]));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const float m2 = mx == -INFINITY ? 0.0f : mx * e.c2;  // the sums are relative to this, rounding and all
+  float s = 0.0f, su = 0.0f;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float u = __builtin_fmaf(acc[i][J][r], e.c2, -m2), w = exp2_(u);
+      s += w;
+      // only columns past the end are -inf among finite ones: 2^-256 is 0
+      su = __builtin_fmaf(w, left < TM * 32 ? fmaxf(u, -256.0f) : u, su);
+    }
+  s += __shfl_xor(s, 32, 64);
+  su += __shfl_xor(su, 32, 64);
+  if (n < N && half == 0) e.row_part[(int64_t)(m0 / (TM * 32)) * N + n] = make_float4(m2, s, su, 0.0f);
+  const int64_t rel = n < N ? e.tokens[n] - m0 : -1;
+  const bool hit = rel >= 0 && rel < TM * 32 && rel < left && ((rel >> 2) & 1) == half;
+  if (__any(hit)) {
+    const float x = find_logit<J, 0, TM>(acc, (int)rel, half);
+    if (hit) e.tok_logit[n] = x;
+  }
+}
+
+// Gradient of the logits of rows n .. n + 31 of h in the 64 vocabulary rows from m0 on, through a 4 KB patch so
+// that whole 128-byte lines leave.
+template <int J, int I0, int TM, int TN>
+__device__ __forceinline__ void dlogits64(const Epilogue& e, const f32x16_v (&acc)[TM][TN], int m0, int M, int nb, int N, int lane,
+                                          unsigned char* patch) {
+  const int half = lane >> 5, l32 = lane & 31, n = nb + l32;
+  const float4 row = e.row_in[n < N ? n : N - 1];
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float d[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float lp = __builtin_fmaf(acc[I0 + i][J][4 * q + t], e.c2, -row.x);
+        d[t] = exp2_(lp) * __builtin_fmaf(row.z, lp, row.y);
+      }
+      *reinterpret_cast<uint2*>(patch + l32 * 128 + (((4 * i + q) ^ (l32 & 7)) << 4) + half * 8) =
+          make_uint2(pack_bf2(d[0], d[1]), pack_bf2(d[2], d[3]));
+    }
+  const int64_t rel = n < N && row.w != 0.0f ? e.tokens[n] - e.col0 - m0 : -1;
+  const bool hit = rel >= 0 && rel < 64 && ((rel >> 2) & 1) == half;
+  wave_lds_fence();
+  if (__any(hit)) {
+    const float x = find_logit<J, I0, 2>(acc, (int)rel, half);
+    const float lp = __builtin_fmaf(x, e.c2, -row.x);
+    if (hit)
+      *reinterpret_cast<bf16*>(patch + l32 * 128 + ((((int)rel >> 3) ^ (l32 & 7)) << 4) + ((int)rel & 7) * 2) =
+          f2bf(__builtin_fmaf(exp2_(lp), __builtin_fmaf(row.z, lp, row.y), row.w));
+    wave_lds_fence();
+  }
+  const int ch = lane & 7, m = m0 + ch * 8;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = u * 8 + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(patch + r * 128 + ((ch ^ (r & 7)) << 4));
+    if (nb + r < N && m < M) *reinterpret_cast<uint4*>(static_cast<bf16*>(e.c) + (int64_t)(nb + r) * e.ldc + m) = v;
+  }
 }
 
 template <int BM, int BN, int WM, int WN, int BK, int ST, bool AT, bool BT, int EPI, int MODE>
@@ -483,6 +528,25 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
   unsigned char* pst = wave < PPS ? st0 : (wave < 2 * PPS ? st1 : (wave < 3 * PPS ? st2 : st3));
   float* pt = reinterpret_cast<float*>(pst + (wave % PPS) * kPatchBytes);
   const int half = lane >> 5, l32 = lane & 31;
+  if constexpr (EPI == EPI_ROW_SUMS || EPI == EPI_DLOGITS) {
+    const int mw = m0 + wm * WTM;
+    if (mw >= mlim) return;
+    static_assert(TN == 2 && (TM == 2 || TM == 4), "two columns of blocks");
+    const int nb = n0 + wn * WTN;
+    if constexpr (EPI == EPI_ROW_SUMS) {
+      row_sums<0>(e, acc, mw, mlim - mw, nb + l32, p.N, half);
+      row_sums<1>(e, acc, mw, mlim - mw, nb + 32 + l32, p.N, half);
+    } else {
+      unsigned char* patch = reinterpret_cast<unsigned char*>(pt);
+      dlogits64<0, 0>(e, acc, mw, mlim, nb, p.N, lane, patch);
+      dlogits64<1, 0>(e, acc, mw, mlim, nb + 32, p.N, lane, patch);
+      if constexpr (TM == 4) {
+        dlogits64<0, 2>(e, acc, mw + 64, mlim, nb, p.N, lane, patch);
+        dlogits64<1, 2>(e, acc, mw + 64, mlim, nb + 32, p.N, lane, patch);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int jp = 0; jp < TN / 2; ++jp) {
     const int nb = n0 + wn * WTN + jp * 64;
@@ -560,15 +624,7 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
             if (e.dw_row && m < mlim && (lane & 7) == 0) e.dw_row[m] = part;
             continue;
           }
-          if constexpr (EPI == EPI_ROW_SUMS) {
-            row_sums8(e, m, mlim, n, p.N, p.M, pt + row * kPatchPitch + cc, lane);
-            continue;
-          }
           if (m >= mlim || n >= p.N) continue;
-          if constexpr (EPI == EPI_DLOGITS) {
-            dlogits8(e, m, n, pt + row * kPatchPitch + cc);
-            continue;
-          }
           if constexpr (EPI == EPI_SWIGLU_BWD && MODE != MODE_GROUP_M) {
             swiglu_bwd8(e, m, n, pt + row * kPatchPitch + cc);
             continue;
@@ -834,6 +890,11 @@ size_t gemm_tile_split_bytes(int M, int N, int K) {
   const int wgrad = tile_splits(M, N, K, true), rows = tile_splits(M, N, K, false);
   const int most = wgrad > rows ? wgrad : rows;
   return most > 1 ? (size_t)most * M * N * sizeof(float) : 0;
+}
+
+int gemm_tile_row_blocks(int M, int N, int K) {
+  const int rows = pick_tile(M, N, K, false, 1, 1).tile / 2;  // both tiles have two waves along m
+  return (M + rows - 1) / rows;
 }
 
 int gemm_tile_launch(const GemmArgs& p0, int epi_kind, hipStream_t stream, int vec, void* ws, size_t ws_bytes,

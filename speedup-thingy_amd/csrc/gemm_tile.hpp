@@ -31,4 +31,7 @@ size_t gemm_tile_split_bytes(int M, int N, int K);
 int gemm_tile_launch(const GemmArgs& p, int epi_kind, hipStream_t stream, int vec, void* ws, size_t ws_bytes,
                      int* splits);
 
+// Blocks of vocabulary rows (one wave's) that EPI_ROW_SUMS leaves sums for.
+int gemm_tile_row_blocks(int M, int N, int K);
+
 }  // namespace rte

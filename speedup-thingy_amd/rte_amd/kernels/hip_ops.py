@@ -1782,7 +1782,7 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         if T == 0:
             dh, dw = hb.new_zeros(hb.shape), wb.new_zeros(wb.shape)
         else:
-            fused = V % 8 == 0 and _lib.load().rte_lm_head_logprobs_ok(T, hb.shape[1], V)
+            fused = _lib.load().rte_lm_head_logprobs_ok(T, hb.shape[1], V)
             grads = LMHeadLogprobsFn._grads if fused else LMHeadLogprobsFn._grads_by_rows
             with _on_device(hb.device):
                 dh, dw = grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_dt == BF16)
@@ -1806,13 +1806,18 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         dw = torch.empty((V, d), dtype=BF16 if w_bf16 else F32, device=dev) if need_w else None
         ws = _scratch(lib.rte_lm_head_dlogits_workspace_bytes(T), dev)
         for lo, hi in zip(cuts, cuts[1:]):
-            dl = torch.empty((T, hi - lo), dtype=BF16, device=dev)
-            call("rte_lm_head_dlogits", ptr(hb), ptr(wb), T, d, V, lo, hi - lo, ptr(tk), temperature, ptr(stats), ptr(ent),
+            wr, n = wb[lo:hi], (hi - lo + 7) // 8 * 8
+            if n > hi - lo:  # rows of zeros, whose gradients add nothing to dh and are dropped from dW
+                wr = torch.nn.functional.pad(wr, (0, 0, 0, n - (hi - lo)))
+            dl = torch.empty((T, n), dtype=BF16, device=dev)
+            call("rte_lm_head_dlogits", ptr(hb), ptr(wr), T, d, V, lo, n, ptr(tk), temperature, ptr(stats), ptr(ent),
                  ptr(gl), ptr(ge), ptr(dl), ptr(ws), ws.numel(), _s())
             if need_h:
-                gemm(dl, wb[lo:hi], b_t=True, out=dh, beta=float(lo > 0))
-            if need_w:
+                gemm(dl, wr, b_t=True, out=dh, beta=float(lo > 0))
+            if need_w and n == hi - lo:
                 gemm(dl, hb, a_t=True, b_t=True, out=dw[lo:hi])
+            elif need_w:
+                dw[lo:hi] = gemm(dl, hb, a_t=True, b_t=True, out_f32=True)[: hi - lo]
         return dh, dw
 
     @staticmethod

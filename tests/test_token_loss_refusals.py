@@ -52,7 +52,7 @@ def test_lm_head_logprobs(lib):
     def bwd(h=BUF, w=BUF, T=100, d=128, V=1000, c=0, n=64, tok=BUF, t=1.0, st=BUF, ent=BUF, dl=BUF, ws=BUF, wsn=room):
         refused(lib, "rte_lm_head_dlogits", h, w, T, d, V, c, n, tok, t, st, ent, BUF, BUF, dl, ws, wsn, None)
 
-    bwd(c=-8), bwd(c=944), bwd(n=0), bwd(n=60), bwd(n=1008), bwd(d=100), bwd(t=-1.0), bwd(st=None), bwd(ent=None)
+    bwd(c=-8), bwd(c=1000), bwd(c=936, n=72), bwd(n=0), bwd(n=60), bwd(n=1008), bwd(d=100), bwd(t=-1.0), bwd(st=None), bwd(ent=None)
     bwd(dl=None), bwd(dl=BUF + 4), bwd(ws=None), bwd(wsn=room - 1), bwd(tok=None), bwd(h=None), bwd(w=None)
 
 
