@@ -48,17 +48,24 @@ struct Row<bf16> {
   }
 };
 
+template <class X>
+__device__ __forceinline__ Words whole_words(const X* at) {
+  const words_v v = *reinterpret_cast<const words_v*>(at);
+  return {{v.x, v.y, v.z, v.w}};
+}
+
 // Elements at .. at + VE of a row that ends at `end`; what lies past the end is -inf.
 template <class X>
 __device__ __forceinline__ Words load_words(const X* row, int at, int end) {
   constexpr int VE = Row<X>::VE;
+  if (at + VE <= end) return whole_words(row + at);
   Words r;
-  if (at + VE <= end) {
-    const words_v v = *reinterpret_cast<const words_v*>(row + at);
-    r = {{v.x, v.y, v.z, v.w}};
-  } else {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) Row<X>::set(r, j, at + j < end ? Row<X>::one(row, at + j) : -INFINITY);
+  for (int j = 0; j < VE; ++j) Row<X>::set(r, j, -INFINITY);
+  if (at < end) {
+#pragma unroll
+    for (int j = 0; j < VE - 1; ++j)
+      if (at + j < end) Row<X>::set(r, j, Row<X>::one(row, at + j));
   }
   return r;
 }

@@ -15,6 +15,8 @@
 #include "../../include/rte_hip.h"
 #include "row_words.hpp"
 
+#include <float.h>
+
 namespace rte {
 
 namespace {
@@ -32,6 +34,27 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k > kInfKey ? 0x7fc00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 __device__ __forceinline__ u64 full_key(float x, int col) { return (u64)value_key(x) << 32 | (uint32_t)~col; }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;  // without the canonical copies that fmaxf makes of operands it knows nothing of
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// Largest of a vector's columns and m (NaN loses).
+template <class X>
+__device__ __forceinline__ float words_max(const Words& v, float m) {
+#pragma unroll
+  for (int j = 0; j < Row<X>::VE; j += 2) m = max3(m, Row<X>::get(v, j), Row<X>::get(v, j + 1));
+  return m;
+}
+
+// Keeps what was computed of these words from being kept too: each phase unpacks them again, for a row's bf16
+// columns as floats take twice the registers of the row.
+template <int N>
+__device__ __forceinline__ void forget(Words (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i].w[0]), "+v"(w[i].w[1]), "+v"(w[i].w[2]), "+v"(w[i].w[3]));
+}
 
 struct RowArgs {
   int64_t ld;
@@ -222,7 +245,7 @@ constexpr int kCandWave = 512, kCandGroup = 1024;
 // of them, go to LDS and each finds its rank there by counting.  Rows whose ties bring more than LDS holds
 // find the n-th value and the last of its columns by bits.
 template <class X, int NW, int E, bool DIST, bool TOP>
-__global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ logits, RowArgs a) {
+__global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_fwd_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, NV = E / VE, NT = 64 * NW, GROUPS = 4 / NW, RPB = 4 / NW;
   constexpr int CAP = NW == 1 ? kCandWave : kCandGroup;
   constexpr int MASKW = NT * E / 32;
@@ -254,7 +277,9 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int off = (i * NT + tid) * VE;
-    if (i * NT * VE < len) {
+    if ((i + 1) * NT * VE <= len) {
+      w[i] = whole_words(at + off);
+    } else if (i * NT * VE < len) {
       w[i] = load_words(at, off, len);
     } else {
 #pragma unroll
@@ -295,8 +320,7 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
     gm[g] = -INFINITY;
 #pragma unroll
     for (int i = g * (NV / GROUPS); i < (g + 1) * (NV / GROUPS); ++i)
-#pragma unroll
-      for (int j = 0; j < VE; ++j) gm[g] = fmaxf(gm[g], Row<X>::get(w[i], j));
+      if (i * NT * VE < len) gm[g] = words_max<X>(w[i], gm[g]);
     m = fmaxf(m, gm[g]);
     gk[g] = value_key(gm[g]);
   }
@@ -334,10 +358,12 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
     }
   }
 
+  forget(w);
   const float m0 = m == -INFINITY ? 0.0f : m;
   float s = 0.0f, su = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    if (i * NT * VE >= len) continue;
 #pragma unroll
     for (int j = 0; j < VE; ++j) {
       const float u = (Row<X>::get(w[i], j) - m0) * a.c2;
@@ -345,6 +371,7 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
       s += e;
       if constexpr (!DIST) su += e * fmaxf(u, -256.0f);  // -inf: e is 0 and the product has to be
     }
+  }
   s = wave_sum(s);
   if constexpr (!DIST) su = wave_sum(su);
   if constexpr (NW > 1) {
@@ -371,10 +398,12 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
     u64* cand = s_cand[slot];
     const float least = key_value(thr);  // not less than it: in (NaN and, where it is NaN, everything in)
     int n = 0;
-    auto collect = [&](auto in) {
+    auto collect = [&](auto any_of, auto in) {
       n = 0;
+      forget(w);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (i * NT * VE >= len || !__any(any_of(w[i]))) continue;
         const int off = (i * NT + tid) * VE;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
@@ -395,21 +424,22 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
       grp.sync();
       if constexpr (NW > 1) n = s_ctl[0];
     };
-    collect([&](float x, int) { return !(x < least); });
+    // a vector is looked into where its maximum passes, or where the row holds NaN (its sum is NaN then)
+    const bool look = s != s;
+    collect([&](const Words& v) { return look || !(words_max<X>(v, -INFINITY) < least); },
+            [&](float x, int) { return !(x < least); });
     if (n > CAP) {
       // value of rank `want`, then the last of its columns that is in
       auto total = [&](auto in) {
         int c = 0;
+        forget(w);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          // a row's keys are made again for every bit: hoisted, they took 241 registers where the row takes 32
-          asm volatile("" : "+v"(w[i].w[0]), "+v"(w[i].w[1]), "+v"(w[i].w[2]), "+v"(w[i].w[3]));
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < VE; ++j) {
             const int rel = (i * NT + tid) * VE + j;
             c += __popcll(__ballot(rel < len && in(value_key(Row<X>::get(w[i], j)), rel)));
           }
-        }
         return grp.count(c);
       };
       uint32_t kth = 0;
@@ -428,23 +458,129 @@ __global__ void __launch_bounds__(256) rows_fwd_kernel(const X* __restrict__ log
         if (tid == 0) s_ctl[0] = 0;
         __syncthreads();
       }
-      collect([&](float x, int rel) {
+      collect([](const Words&) { return true; }, [&](float x, int rel) {
         const uint32_t k = value_key(x);
         return k > kth || (k == kth && rel <= last);
       });
     }
     if (tid < 2) cand[n + tid] = 0;
     grp.sync();
-    for (int c = tid; c < n; c += NT) {
-      const u64 mine = cand[c];
-      int rank = 0;
-      for (int j = 0; j < n; j += 2) rank += (cand[j] > mine) + (cand[j + 1] > mine);
-      if (rank >= want) continue;
-      if (NW > 1 && a.nparts > 1) a.part_keys[(t * a.nparts + p) * want + rank] = mine;
-      else put_top(a, t, rank, mine, r);
+    for (int c = tid; c < n; c += 2 * NT) {  // two candidates a pass
+      const u64 mine[2] = {cand[c], c + NT < n ? cand[c + NT] : ~0ull};
+      int rank[2] = {0, 0};
+      for (int j = 0; j < n; j += 2) {
+        const u64 x = cand[j], y = cand[j + 1];
+        rank[0] += (x > mine[0]) + (y > mine[0]);
+        rank[1] += (x > mine[1]) + (y > mine[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (c + i * NT >= n || rank[i] >= want) continue;
+        if (NW > 1 && a.nparts > 1) a.part_keys[(t * a.nparts + p) * want + rank[i]] = mine[i];
+        else put_top(a, t, rank[i], mine[i], r);
+      }
     }
     if (NW > 1 && a.nparts > 1)  // a short last range
       for (int c = n + tid; c < want; c += NT) a.part_keys[(t * a.nparts + p) * want + c] = 0;
+  }
+}
+
+// A range of a row in one pass of a workgroup, for rows of which only the sums are wanted: every lane keeps its
+// own running maximum and sums over batches of four vectors, the next of them on its way, and nothing is
+// exchanged before the end.  Columns listed (DIST) are left out by a bit mask in LDS.
+constexpr int kBatch = 4;
+constexpr int kStreamCols = 65536;  // of the bit mask, 8 KB
+template <class X, bool DIST>
+__global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict__ logits, RowArgs a) {
+  constexpr int VE = Row<X>::VE, COLS = kBatch * 256 * VE;
+  __shared__ uint32_t s_mask[DIST ? kStreamCols / 32 : 1];
+  __shared__ Sums s_sums[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t = blockIdx.x / (unsigned)a.nparts;
+  const int p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
+  const X* row = logits + t * a.ld;
+  const int c0 = p * a.part;
+  const int len = a.V - c0 < a.part ? a.V - c0 : a.part;
+  const X* at = row + c0;
+  auto load = [&](int b, Words* to) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int off = b + (i * 256 + tid) * VE;
+      if (b + COLS <= len) to[i] = whole_words(at + off);
+      else to[i] = load_words(at, off, len);
+    }
+  };
+  Words next[kBatch];
+  load(0, next);
+  bool unique = true;
+  if constexpr (DIST) {
+    for (int i = tid; i < (len + 31) / 32; i += 256) s_mask[i] = 0;
+    __syncthreads();
+    bool again = false;
+    if (tid < a.K) {
+      const int id = a.ids[t * a.K + tid], rel = id - c0;
+      if (id >= c0 && rel < len) again = (atomicOr(&s_mask[rel >> 5], 1u << (rel & 31)) >> (rel & 31)) & 1;
+    }
+    unique = __syncthreads_or(again) == 0;
+  }
+  Sums r{-FLT_MAX, 0.0f, 0.0f};  // a lowest maximum: -inf columns add nothing, lowest ones count
+  for (int b = 0; b < len; b += COLS) {
+    Words w[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) w[i] = next[i];
+    if (b + COLS < len) load(b + COLS, next);
+    if constexpr (DIST) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int off = b + (i * 256 + tid) * VE;
+        const uint32_t bits = off < len ? s_mask[off >> 5] >> (off & 31) & ((1u << VE) - 1) : 0;
+        if (bits) {
+#pragma unroll
+          for (int j = 0; j < VE; ++j)
+            if (bits >> j & 1) Row<X>::set(w[i], j, -INFINITY);
+        }
+      }
+    }
+    float m = r.m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) m = words_max<X>(w[i], m);
+    const float d = (r.m - m) * a.c2, scale = exp2_(d);
+    if constexpr (!DIST) r.su = scale * (r.su + r.s * fmaxf(d, -256.0f));
+    r.s *= scale;
+    r.m = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const float u = (Row<X>::get(w[i], j) - m) * a.c2, e = exp2_(u);
+        r.s += e;
+        if constexpr (!DIST) r.su += e * fmaxf(u, -256.0f);
+      }
+  }
+  auto join = [&](const Sums& x, float top) {  // x relative to top
+    const float d = (x.m - top) * a.c2, e = exp2_(d);
+    return Sums{top, x.s != x.s ? x.s : x.s * e, e * (x.su + x.s * fmaxf(d, -256.0f))};
+  };
+  r = join(r, wave_max(r.m));
+  r.s = wave_sum(r.s);
+  r.su = wave_sum(r.su);
+  if (lane == 0) s_sums[wave] = r;
+  __syncthreads();
+  if (wave != 0) return;
+  const float top = fmaxf(fmaxf(s_sums[0].m, s_sums[1].m), fmaxf(s_sums[2].m, s_sums[3].m));
+  r = join(s_sums[0], top);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const Sums o = join(s_sums[i], top);
+    r.s += o.s;
+    r.su += o.su;
+  }
+  if (a.nparts > 1) {
+    if (lane == 0) a.part_stats[t * a.nparts + p] = make_float4(r.m, r.s, r.su, 0.0f);
+  } else if constexpr (DIST) {
+    finish_distill(a, row, t, r, unique, lane);
+  } else {
+    if (lane == 0) finish_logprobs(a, row, t, r);
   }
 }
 
@@ -592,17 +728,14 @@ __global__ void __launch_bounds__(256)
     if (here[i]) Row<X>::put(out, col[i], gt * cf[i]);
 }
 
-// Ranges of a row.  One wave holds up to 2048 columns, a workgroup 16384; longer rows are cut, and so are
-// rows too few to give the chip's CUs work, down to 2048 columns.
-int parts_of(int T, int V) {
-  if (V <= kRowCols) return 1;
-  const int least = (V + 16383) / 16384, most = (V + 2047) / 2048;
+// Ranges of a row.  Of a row with alternatives a workgroup holds up to 16384 columns; of others it streams up to
+// kStreamCols.  Rows too few to give the chip's CUs work are cut further, down to 2048 and 8192 columns.
+int part_len(int T, int V, bool top) {
+  const int hold = top ? 16384 : kStreamCols, fine = top ? 2048 : 8192;
+  const int least = (V + hold - 1) / hold, most = (V + fine - 1) / fine;
   const int wanted = (512 + T - 1) / T;
-  return wanted < least ? least : wanted > most ? most : wanted;
-}
-int part_len(int T, int V) {
-  const int n = parts_of(T, V);
-  return ((V + n - 1) / n + 255) / 256 * 256;
+  const int n = wanted < least ? least : wanted > most ? most : wanted;
+  return ((V + n - 1) / n + 2047) / 2048 * 2048;
 }
 
 template <class X, bool DIST, bool TOP>
@@ -614,16 +747,20 @@ int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((rows_fwd_kernel<X, 1, kRowCols / 64, DIST, TOP>), dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
     return check_launch("token_loss_rows");
   }
-  a.part = part_len(a.T, a.V);
+  a.part = part_len(a.T, a.V, TOP);
   a.nparts = (a.V + a.part - 1) / a.part;
   const int64_t grid = (int64_t)a.T * a.nparts;
   RTE_REQUIRE(grid < ((int64_t)1 << 31), "token_loss: too many rows");
   a.part_stats = static_cast<float4*>(ws);
   a.part_keys = reinterpret_cast<u64*>(a.part_stats + grid);
-  auto fn = a.part <= 4096   ? rows_fwd_kernel<X, 4, 16, DIST, TOP>
-            : a.part <= 8192 ? rows_fwd_kernel<X, 4, 32, DIST, TOP>
-                             : rows_fwd_kernel<X, 4, 64, DIST, TOP>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  if constexpr (TOP) {
+    auto fn = a.part <= 4096   ? rows_fwd_kernel<X, 4, 16, DIST, TOP>
+              : a.part <= 8192 ? rows_fwd_kernel<X, 4, 32, DIST, TOP>
+                               : rows_fwd_kernel<X, 4, 64, DIST, TOP>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  } else {
+    hipLaunchKernelGGL((rows_stream_kernel<X, DIST>), dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  }
   RTE_TRY(check_launch("token_loss_rows"));
   if (a.nparts == 1) return 0;
   hipLaunchKernelGGL((rows_join_kernel<X, DIST, TOP>), dim3(a.T), dim3(TOP ? 256 : 64), 0, s, x, a);
@@ -632,7 +769,7 @@ int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
 
 size_t rows_workspace(int T, int V, int n_top) {
   if (T <= 0 || V <= kRowCols) return 0;
-  const int part = part_len(T, V), n = (V + part - 1) / part;
+  const int part = part_len(T, V, n_top > 0), n = (V + part - 1) / part;
   return n > 1 ? (size_t)T * n * (sizeof(float4) + n_top * sizeof(u64)) : 0;
 }
 
