@@ -210,77 +210,71 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   }
 }
 
-// Threads that share a row (or a range of one): one wave, or the four of a workgroup.
-template <int NW>
-struct Group {
-  static constexpr int NT = 64 * NW;
-  float* red;  // [3 * NW]
-  int tid, wave;
-  __device__ __forceinline__ void sync() const {
-    if constexpr (NW == 1) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    } else {
-      __syncthreads();
+// Rank of every candidate among the n in LDS (two places past them are written) by counting the larger keys,
+// two candidates a pass; those of rank below `want` go to put(rank, key).
+template <int NT, class P>
+__device__ __forceinline__ void rank_keys(u64* cand, int n, int want, int tid, P put) {
+  for (int c = tid; c < n; c += 2 * NT) {
+    const u64 mine[2] = {cand[c], c + NT < n ? cand[c + NT] : ~0ull};
+    int rank[2] = {0, 0};
+    for (int j = 0; j < n; j += 2) {
+      const u64 x = cand[j], y = cand[j + 1];
+      rank[0] += (x > mine[0]) + (y > mine[0]);
+      rank[1] += (x > mine[1]) + (y > mine[1]);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c + i * NT < n && rank[i] < want) put(rank[i], mine[i]);
   }
-  // total of a per-wave count (uniform in the wave)
-  __device__ int count(int n) const {
-    if constexpr (NW == 1) return n;
-    __syncthreads();
-    if ((tid & 63) == 0) reinterpret_cast<int*>(red)[wave] = n;
-    __syncthreads();
-    int s = 0;
-    for (int i = 0; i < NW; ++i) s += reinterpret_cast<int*>(red)[i];
-    return s;
+}
+
+// The want-th largest of 256 keys (four per lane), to its leading bits above bit `low`: at least `want` keys are
+// not below the result.
+__device__ __forceinline__ uint32_t nth_key(const uint32_t* k, int want, int low, bool exact) {
+  uint32_t thr = 0;
+  for (int b = 31; b >= low; --b) {
+    const uint32_t c = thr | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) n += __popcll(__ballot(k[g] >= c));
+    if (n >= want) thr = c;
+    if (n == want && !exact) break;
   }
-};
+  return thr;
+}
 
 constexpr int kRowCols = 2048;  // columns of a row that one wave holds
 constexpr int kCandWave = 512, kCandGroup = 1024;
 
-// One pass over a row (or one of its ranges), held in registers: E columns per thread.  The maximum comes
-// first, so no sum is rescaled.  For the alternatives, the n-th largest of 256 maxima (of a thread's
-// columns, or quarters of them) is a threshold that n columns reach at least; those that do, about n ln(...)
-// of them, go to LDS and each finds its rank there by counting.  Rows whose ties bring more than LDS holds
-// find the n-th value and the last of its columns by bits.
-template <class X, int NW, int E, bool DIST, bool TOP>
-__global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_fwd_kernel(const X* __restrict__ logits, RowArgs a) {
-  constexpr int VE = Row<X>::VE, NV = E / VE, NT = 64 * NW, GROUPS = 4 / NW, RPB = 4 / NW;
-  constexpr int CAP = NW == 1 ? kCandWave : kCandGroup;
-  constexpr int MASKW = NT * E / 32;
-  static_assert(NV * VE == E && NV >= GROUPS && NV % GROUPS == 0, "whole vectors, a group of them each");
-  __shared__ float s_red[RPB][3 * NW];
-  __shared__ uint32_t s_mask[DIST ? RPB : 1][DIST ? MASKW : 1];
-  __shared__ u64 s_cand[TOP ? RPB : 1][TOP ? CAP + 2 : 1];
-  __shared__ uint32_t s_gmax[TOP && NW > 1 ? 256 : 1];
-  __shared__ int s_ctl[2];  // candidates, threshold
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A short row by one wave, held in registers: E columns per lane, read once.  The maximum comes first, so no
+// sum is rescaled.  For the alternatives, the n-th largest of 256 maxima (of quarters of the lanes' columns) is
+// a threshold that n columns reach at least; those that do go to LDS and each finds its rank there.  Rows whose
+// ties bring more than LDS holds find the n-th value and the last of its columns by bits.
+template <class X, int E, bool DIST, bool TOP>
+__global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
+  constexpr int VE = Row<X>::VE, NV = E / VE, COLS = 64 * VE;
+  static_assert(NV * VE == E && NV >= 4 && NV % 4 == 0, "whole vectors, four groups of them");
+  __shared__ uint32_t s_mask[DIST ? 4 : 1][DIST ? 2 * E : 1];
+  __shared__ u64 s_cand[TOP ? 4 : 1][TOP ? kCandWave + 2 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slot = NW == 1 ? wave : 0;
-  Group<NW> grp{s_red[slot], NW == 1 ? lane : (int)threadIdx.x, NW == 1 ? 0 : wave};
-  const int tid = grp.tid;
-  int64_t t;
-  int p = 0;
-  if constexpr (NW == 1) {
-    t = (int64_t)blockIdx.x * 4 + wave;
-    if (t >= a.T) return;
-  } else {
-    t = blockIdx.x / (unsigned)a.nparts;
-    p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
-  }
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= a.T) return;
   const X* row = logits + t * a.ld;
-  const int c0 = p * a.part;
-  const int len = a.V - c0 < a.part ? a.V - c0 : a.part;
-  const X* at = row + c0;
+  const int len = a.V;
 
   Words w[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int off = (i * NT + tid) * VE;
-    if ((i + 1) * NT * VE <= len) {
-      w[i] = whole_words(at + off);
-    } else if (i * NT * VE < len) {
-      w[i] = load_words(at, off, len);
+    const int off = (i * 64 + lane) * VE;
+    if ((i + 1) * COLS <= len) {
+      w[i] = whole_words(row + off);
+    } else if (i * COLS < len) {
+      w[i] = load_words(row, off, len);
     } else {
 #pragma unroll
       for (int j = 0; j < VE; ++j) Row<X>::set(w[i], j, -INFINITY);
@@ -289,19 +283,19 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
 
   bool unique = true;
   if constexpr (DIST) {
-    uint32_t* mask = s_mask[slot];
-    for (int i = tid; i < MASKW; i += NT) mask[i] = 0;
-    grp.sync();
+    uint32_t* mask = s_mask[wave];
+    for (int i = lane; i < 2 * E; i += 64) mask[i] = 0;
+    wave_fence();
     bool again = false;
-    for (int j = tid; j < a.K; j += NT) {
-      const int id = a.ids[t * a.K + j], rel = id - c0;
-      if (id >= c0 && rel < len) again |= (atomicOr(&mask[rel >> 5], 1u << (rel & 31)) >> (rel & 31)) & 1;
+    for (int j = lane; j < a.K; j += 64) {
+      const int id = a.ids[t * a.K + j];
+      if (id >= 0 && id < len) again |= (atomicOr(&mask[id >> 5], 1u << (id & 31)) >> (id & 31)) & 1;
     }
-    unique = !__any(again);  // as far as this wave sees: of NW > 1, entries 64 wave .. 64 wave + 63
-    grp.sync();
+    unique = !__any(again);
+    wave_fence();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int off = (i * NT + tid) * VE;
+      const int off = (i * 64 + lane) * VE;
       const uint32_t bits = mask[off >> 5] >> (off & 31) & ((1u << VE) - 1);
       if (bits) {
 #pragma unroll
@@ -312,58 +306,28 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
   }
 
   // maxima (a NaN column shows in the sums)
-  float gm[GROUPS];
-  uint32_t gk[GROUPS];
+  uint32_t gk[4];
   float m = -INFINITY;
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    gm[g] = -INFINITY;
+  for (int g = 0; g < 4; ++g) {
+    float gm = -INFINITY;
 #pragma unroll
-    for (int i = g * (NV / GROUPS); i < (g + 1) * (NV / GROUPS); ++i)
-      if (i * NT * VE < len) gm[g] = words_max<X>(w[i], gm[g]);
-    m = fmaxf(m, gm[g]);
-    gk[g] = value_key(gm[g]);
+    for (int i = g * (NV / 4); i < (g + 1) * (NV / 4); ++i)
+      if (i * COLS < len) gm = words_max<X>(w[i], gm);
+    m = fmaxf(m, gm);
+    gk[g] = value_key(gm);
   }
   m = wave_max(m);
-  if constexpr (NW > 1) {
-    if (lane == 0) grp.red[wave] = m;
-    if constexpr (TOP) s_gmax[tid] = gk[0];
-    if (tid == 0) s_ctl[0] = 0;
-    __syncthreads();
-    m = fmaxf(fmaxf(grp.red[0], grp.red[1]), fmaxf(grp.red[2], grp.red[3]));
-  }
-
-  // threshold: the want-th largest of 256 maxima, to the leading bits (16 of them are all of a bf16 value)
-  const int want = a.n_top;
   uint32_t thr = 0;
-  if constexpr (TOP) {
-    if (NW == 1 || wave == 0) {
-      uint32_t k[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if constexpr (NW == 1) k[g] = gk[g];
-        else k[g] = s_gmax[lane + 64 * g];
-      }
-      for (int b = 31; b >= (VE == 8 ? 16 : 12); --b) {
-        const uint32_t c = thr | 1u << b;
-        int n = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) n += __popcll(__ballot(k[g] >= c));
-        if (n >= want) thr = c;
-        if (n == want) break;
-      }
-      if constexpr (NW > 1) {
-        if (lane == 0) s_ctl[1] = (int)thr;
-      }
-    }
-  }
+  const int want = a.n_top;
+  if constexpr (TOP) thr = nth_key(gk, want, VE == 8 ? 16 : 12, false);  // 16 bits are all of a bf16 value
 
   forget(w);
   const float m0 = m == -INFINITY ? 0.0f : m;
   float s = 0.0f, su = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i * NT * VE >= len) continue;
+    if (i * COLS >= len) continue;
 #pragma unroll
     for (int j = 0; j < VE; ++j) {
       const float u = (Row<X>::get(w[i], j) - m0) * a.c2;
@@ -374,28 +338,15 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
   }
   s = wave_sum(s);
   if constexpr (!DIST) su = wave_sum(su);
-  if constexpr (NW > 1) {
-    if (lane == 0) {
-      grp.red[NW + wave] = s;
-      grp.red[2 * NW + wave] = su;
-    }
-    __syncthreads();
-    s = (grp.red[NW] + grp.red[NW + 1]) + (grp.red[NW + 2] + grp.red[NW + 3]);
-    su = (grp.red[2 * NW] + grp.red[2 * NW + 1]) + (grp.red[2 * NW + 2] + grp.red[2 * NW + 3]);
-    if constexpr (TOP) thr = (uint32_t)s_ctl[1];
-  }
   const Sums r{m, s, su};
-
-  if (NW > 1 && a.nparts > 1) {
-    if (tid == 0) a.part_stats[t * a.nparts + p] = make_float4(m, s, su, 0.0f);
-  } else if constexpr (DIST) {
-    if (NW == 1 || wave == 0) finish_distill(a, row, t, r, unique && (NW == 1 || a.K <= 64), lane);
+  if constexpr (DIST) {
+    finish_distill(a, row, t, r, unique, lane);
   } else {
-    if (tid == 0) finish_logprobs(a, row, t, r);
+    if (lane == 0) finish_logprobs(a, row, t, r);
   }
 
   if constexpr (TOP) {
-    u64* cand = s_cand[slot];
+    u64* cand = s_cand[wave];
     const float least = key_value(thr);  // not less than it: in (NaN and, where it is NaN, everything in)
     int n = 0;
     auto collect = [&](auto any_of, auto in) {
@@ -403,32 +354,26 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
       forget(w);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (i * NT * VE >= len || !__any(any_of(w[i]))) continue;
-        const int off = (i * NT + tid) * VE;
+        if (i * COLS >= len || !__any(any_of(w[i]))) continue;
+        const int off = (i * 64 + lane) * VE;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           const float x = Row<X>::get(w[i], j);
           const bool here = in(x, off + j) && off + j < len;
           const u64 who = __ballot(here);
           if (who == 0) continue;
-          int base = n;
-          if constexpr (NW > 1) {
-            if (lane == 0) base = atomicAdd(&s_ctl[0], __popcll(who));
-            base = __builtin_amdgcn_readfirstlane(base);
-          }
-          const int pos = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-          if (here && pos < CAP) cand[pos] = full_key(x, c0 + off + j);
+          const int pos = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+          if (here && pos < kCandWave) cand[pos] = full_key(x, off + j);
           n += __popcll(who);
         }
       }
-      grp.sync();
-      if constexpr (NW > 1) n = s_ctl[0];
+      wave_fence();
     };
     // a vector is looked into where its maximum passes, or where the row holds NaN (its sum is NaN then)
     const bool look = s != s;
     collect([&](const Words& v) { return look || !(words_max<X>(v, -INFINITY) < least); },
             [&](float x, int) { return !(x < least); });
-    if (n > CAP) {
+    if (n > kCandWave) {
       // value of rank `want`, then the last of its columns that is in
       auto total = [&](auto in) {
         int c = 0;
@@ -437,10 +382,10 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < VE; ++j) {
-            const int rel = (i * NT + tid) * VE + j;
-            c += __popcll(__ballot(rel < len && in(value_key(Row<X>::get(w[i], j)), rel)));
+            const int at = (i * 64 + lane) * VE + j;
+            c += __popcll(__ballot(at < len && in(value_key(Row<X>::get(w[i], j)), at)));
           }
-        return grp.count(c);
+        return c;
       };
       uint32_t kth = 0;
       for (int b = 31; b >= 0; --b) {
@@ -449,52 +394,40 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
       }
       const int need = want - total([&](uint32_t k, int) { return k > kth; });
       int last = 0;
-      for (int b = 13; b >= 0; --b) {
+      for (int b = 11; b >= 0; --b) {
         const int c = last | 1 << b;
-        if (total([&](uint32_t k, int rel) { return k == kth && rel < c; }) < need) last = c;
+        if (total([&](uint32_t k, int at) { return k == kth && at < c; }) < need) last = c;
       }
-      if (NW > 1) {
-        __syncthreads();
-        if (tid == 0) s_ctl[0] = 0;
-        __syncthreads();
-      }
-      collect([](const Words&) { return true; }, [&](float x, int rel) {
+      collect([](const Words&) { return true; }, [&](float x, int at) {
         const uint32_t k = value_key(x);
-        return k > kth || (k == kth && rel <= last);
+        return k > kth || (k == kth && at <= last);
       });
     }
-    if (tid < 2) cand[n + tid] = 0;
-    grp.sync();
-    for (int c = tid; c < n; c += 2 * NT) {  // two candidates a pass
-      const u64 mine[2] = {cand[c], c + NT < n ? cand[c + NT] : ~0ull};
-      int rank[2] = {0, 0};
-      for (int j = 0; j < n; j += 2) {
-        const u64 x = cand[j], y = cand[j + 1];
-        rank[0] += (x > mine[0]) + (y > mine[0]);
-        rank[1] += (x > mine[1]) + (y > mine[1]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (c + i * NT >= n || rank[i] >= want) continue;
-        if (NW > 1 && a.nparts > 1) a.part_keys[(t * a.nparts + p) * want + rank[i]] = mine[i];
-        else put_top(a, t, rank[i], mine[i], r);
-      }
-    }
-    if (NW > 1 && a.nparts > 1)  // a short last range
-      for (int c = n + tid; c < want; c += NT) a.part_keys[(t * a.nparts + p) * want + c] = 0;
+    if (lane < 2) cand[n + lane] = 0;
+    wave_fence();
+    rank_keys<64>(cand, n, want, lane, [&](int rank, u64 key) { put_top(a, t, rank, key, r); });
   }
 }
 
-// A range of a row in one pass of a workgroup, for rows of which only the sums are wanted: every lane keeps its
-// own running maximum and sums over batches of four vectors, the next of them on its way, and nothing is
-// exchanged before the end.  Columns listed (DIST) are left out by a bit mask in LDS.
+// A range of a longer row in one pass of a workgroup: every lane keeps its own running maximum and sums over
+// batches of four vectors, the next of them on its way, and nothing is exchanged before the end.  Columns listed
+// (DIST) are left out by a bit mask in LDS.  For the alternatives (TOP) each lane leaves its maximum of every
+// batch in LDS; at the end the n-th largest of the 256 lanes' maxima is a threshold that n columns reach at
+// least, and only the few batches whose maximum reaches it are read again, four lanes each.
 constexpr int kBatch = 4;
-constexpr int kStreamCols = 65536;  // of the bit mask, 8 KB
-template <class X, bool DIST>
+constexpr int kStreamCols = 65536;  // columns of a workgroup: 8 KB of bit mask, 16 batches of fp32
+constexpr int kItems = 512;
+
+template <class X, bool DIST, bool TOP>
 __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, COLS = kBatch * 256 * VE;
   __shared__ uint32_t s_mask[DIST ? kStreamCols / 32 : 1];
   __shared__ Sums s_sums[4];
+  __shared__ float s_bmax[TOP ? kStreamCols / COLS : 1][TOP ? 256 : 1];
+  __shared__ uint32_t s_key[TOP ? 256 : 1];
+  __shared__ u64 s_cand[TOP ? kCandGroup + 2 : 1];
+  __shared__ int s_items[TOP ? kItems : 1];
+  __shared__ int s_ctl[4];  // items, candidates, threshold
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t = blockIdx.x / (unsigned)a.nparts;
   const int p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
@@ -524,6 +457,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     unique = __syncthreads_or(again) == 0;
   }
   Sums r{-FLT_MAX, 0.0f, 0.0f};  // a lowest maximum: -inf columns add nothing, lowest ones count
+  float most = -INFINITY;        // largest entry of s_bmax of this lane
   for (int b = 0; b < len; b += COLS) {
     Words w[kBatch];
 #pragma unroll
@@ -541,21 +475,31 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
         }
       }
     }
-    float m = r.m;
+    float bm = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) m = words_max<X>(w[i], m);
-    const float d = (r.m - m) * a.c2, scale = exp2_(d);
+    for (int i = 0; i < kBatch; ++i)
+      if (b + i * 256 * VE < len) bm = words_max<X>(w[i], bm);
+    const float m = fmaxf(r.m, bm), d = (r.m - m) * a.c2, scale = exp2_(d);
     if constexpr (!DIST) r.su = scale * (r.su + r.s * fmaxf(d, -256.0f));
     r.s *= scale;
     r.m = m;
+    float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
+    for (int i = 0; i < kBatch; ++i) {
+      if (b + i * 256 * VE >= len) continue;
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
         const float u = (Row<X>::get(w[i], j) - m) * a.c2, e = exp2_(u);
-        r.s += e;
+        s += e;
         if constexpr (!DIST) r.su += e * fmaxf(u, -256.0f);
       }
+    }
+    r.s += s;
+    if constexpr (TOP) {
+      bm = s != s ? INFINITY : bm;  // a batch with NaN is always looked into
+      s_bmax[b / COLS][tid] = bm;
+      most = fmaxf(most, bm);
+    }
   }
   auto join = [&](const Sums& x, float top) {  // x relative to top
     const float d = (x.m - top) * a.c2, e = exp2_(d);
@@ -565,8 +509,17 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   r.s = wave_sum(r.s);
   r.su = wave_sum(r.su);
   if (lane == 0) s_sums[wave] = r;
+  if constexpr (TOP) {
+    s_key[tid] = value_key(most);
+    if (tid < 2) s_ctl[tid] = 0;
+  }
   __syncthreads();
-  if (wave != 0) return;
+  const int want = a.n_top;
+  uint32_t keys[4];
+  if constexpr (TOP) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) keys[g] = s_key[lane + 64 * g];
+  }
   const float top = fmaxf(fmaxf(s_sums[0].m, s_sums[1].m), fmaxf(s_sums[2].m, s_sums[3].m));
   r = join(s_sums[0], top);
 #pragma unroll
@@ -575,12 +528,128 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     r.s += o.s;
     r.su += o.su;
   }
-  if (a.nparts > 1) {
-    if (lane == 0) a.part_stats[t * a.nparts + p] = make_float4(r.m, r.s, r.su, 0.0f);
-  } else if constexpr (DIST) {
-    finish_distill(a, row, t, r, unique, lane);
-  } else {
-    if (lane == 0) finish_logprobs(a, row, t, r);
+  if (wave == 0) {
+    if constexpr (TOP) {
+      const uint32_t thr = nth_key(keys, want, VE == 8 ? 16 : 12, false);
+      if (lane == 0) s_ctl[2] = (int)thr;
+    }
+    if (a.nparts > 1) {
+      if (lane == 0) a.part_stats[t * a.nparts + p] = make_float4(r.m, r.s, r.su, 0.0f);
+    } else if constexpr (DIST) {
+      finish_distill(a, row, t, r, unique, lane);
+    } else {
+      if (lane == 0) finish_logprobs(a, row, t, r);
+    }
+  }
+  if constexpr (TOP) {
+    __syncthreads();
+    const float least = key_value((uint32_t)s_ctl[2]);  // not less than it: in (NaN and, where it is NaN, everything in)
+    auto add = [&](float x, int off) {
+      const int pos = atomicAdd(&s_ctl[1], 1);
+      if (pos < kCandGroup) s_cand[pos] = full_key(x, c0 + off);
+    };
+    if (!(most < least)) {
+      for (int b = 0; b * COLS < len; ++b)
+        if (!(s_bmax[b][tid] < least)) {
+          const int pos = atomicAdd(&s_ctl[0], 1);
+          if (pos < kItems) s_items[pos] = b * 256 + tid;
+        }
+    }
+    __syncthreads();
+    const int items = s_ctl[0];
+    if (items <= kItems) {
+      for (int q = tid; q < items * kBatch; q += 256) {
+        const int it = s_items[q / kBatch], off = (it >> 8) * COLS + ((q % kBatch) * 256 + (it & 255)) * VE;
+        const Words v = load_words(at, off, len);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const float x = Row<X>::get(v, j);
+          if (!(x < least) && off + j < len) add(x, off + j);
+        }
+      }
+      __syncthreads();
+    }
+    int n = s_ctl[1];
+    if (items > kItems || n > kCandGroup) {  // ties, or a row whose large values sit in few lanes
+      auto every = [&](auto f) {
+        for (int off = tid * VE; off < len; off += 256 * VE) {
+          const Words v = load_words(at, off, len);
+#pragma unroll
+          for (int j = 0; j < VE; ++j)
+            if (off + j < len) f(Row<X>::get(v, j), off + j);
+        }
+      };
+      auto total = [&](int c) {
+        c = wave_sum(c);
+        __syncthreads();
+        if (lane == 0) s_items[wave] = c;
+        __syncthreads();
+        return (s_items[0] + s_items[1]) + (s_items[2] + s_items[3]);
+      };
+      auto above = [&](uint32_t k) {
+        int c = 0;
+        every([&](float x, int) { c += value_key(x) > k; });
+        return total(c);
+      };
+      // the value of rank `want`: the lanes' own want-th maximum where fewer columns exceed it, else by bits above it
+      uint32_t kth = nth_key(keys, want, 0, true);
+      int over = above(kth);
+      if (over >= want) {
+        const uint32_t floor = kth;
+        kth = 0;
+        for (int b = 31; b >= 0; --b) {
+          const uint32_t c = kth | 1u << b;
+          if (c <= floor || above(c - 1) >= want) kth = c;
+        }
+        over = above(kth);
+      }
+      __syncthreads();
+      if (tid == 0) s_ctl[1] = 0;
+      __syncthreads();
+      every([&](float x, int off) {
+        if (value_key(x) > kth) add(x, off);
+      });
+      // and the first columns that hold that value
+      int left = want - over;
+      for (int off = tid * VE, b = 0; b < len && left > 0; off += 256 * VE, b += 256 * VE) {
+        const Words v = load_words(at, off, len);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) c += off + j < len && value_key(Row<X>::get(v, j)) == kth;
+        int before = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int y = __shfl_up(before, o, 64);
+          if (lane >= o) before += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_items[wave] = before;
+        __syncthreads();
+        before -= c;
+        int all = 0;
+        for (int i = 0; i < 4; ++i) {
+          if (i < wave) before += s_items[i];
+          all += s_items[i];
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const float x = Row<X>::get(v, j);
+          if (off + j < len && value_key(x) == kth && before++ < left) add(x, off + j);
+        }
+        left -= all;
+      }
+      __syncthreads();
+      n = s_ctl[1];
+    }
+    if (tid < 2) s_cand[n + tid] = 0;
+    __syncthreads();
+    u64* out = a.part_keys + (t * a.nparts + p) * want;
+    rank_keys<256>(s_cand, n, want, tid, [&](int rank, u64 key) {
+      if (a.nparts > 1) out[rank] = key;
+      else put_top(a, t, rank, key, r);
+    });
+    if (a.nparts > 1)  // a short last range
+      for (int c = n + tid; c < want; c += 256) out[c] = 0;
   }
 }
 
@@ -728,11 +797,10 @@ __global__ void __launch_bounds__(256)
     if (here[i]) Row<X>::put(out, col[i], gt * cf[i]);
 }
 
-// Ranges of a row.  Of a row with alternatives a workgroup holds up to 16384 columns; of others it streams up to
-// kStreamCols.  Rows too few to give the chip's CUs work are cut further, down to 2048 and 8192 columns.
-int part_len(int T, int V, bool top) {
-  const int hold = top ? 16384 : kStreamCols, fine = top ? 2048 : 8192;
-  const int least = (V + hold - 1) / hold, most = (V + fine - 1) / fine;
+// Ranges of a row of more than kRowCols columns: a workgroup takes up to kStreamCols, and rows too few to give
+// every CU two workgroups are cut further, down to 8192 columns.
+int part_len(int T, int V) {
+  const int least = (V + kStreamCols - 1) / kStreamCols, most = (V + 8191) / 8192;
   const int wanted = (512 + T - 1) / T;
   const int n = wanted < least ? least : wanted > most ? most : wanted;
   return ((V + n - 1) / n + 2047) / 2048 * 2048;
@@ -742,26 +810,17 @@ template <class X, bool DIST, bool TOP>
 int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
   const X* x = static_cast<const X*>(logits);
   if (a.V <= kRowCols) {
-    a.nparts = 1;
-    a.part = kRowCols;
-    hipLaunchKernelGGL((rows_fwd_kernel<X, 1, kRowCols / 64, DIST, TOP>), dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
+    hipLaunchKernelGGL((rows_wave_kernel<X, kRowCols / 64, DIST, TOP>), dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
     return check_launch("token_loss_rows");
   }
-  a.part = part_len(a.T, a.V, TOP);
+  a.part = part_len(a.T, a.V);
   a.nparts = (a.V + a.part - 1) / a.part;
   const int64_t grid = (int64_t)a.T * a.nparts;
   RTE_REQUIRE(grid < ((int64_t)1 << 31), "token_loss: too many rows");
   a.part_stats = static_cast<float4*>(ws);
   a.part_keys = reinterpret_cast<u64*>(a.part_stats + grid);
-  if constexpr (TOP) {
-    auto fn = a.part <= 4096   ? rows_fwd_kernel<X, 4, 16, DIST, TOP>
-              : a.part <= 8192 ? rows_fwd_kernel<X, 4, 32, DIST, TOP>
-                               : rows_fwd_kernel<X, 4, 64, DIST, TOP>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(256), 0, s, x, a);
-  } else {
-    hipLaunchKernelGGL((rows_stream_kernel<X, DIST>), dim3((unsigned)grid), dim3(256), 0, s, x, a);
-  }
-  RTE_TRY(check_launch("token_loss_rows"));
+  hipLaunchKernelGGL((rows_stream_kernel<X, DIST, TOP>), dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  RTE_TRY(check_launch("token_loss_stream"));
   if (a.nparts == 1) return 0;
   hipLaunchKernelGGL((rows_join_kernel<X, DIST, TOP>), dim3(a.T), dim3(TOP ? 256 : 64), 0, s, x, a);
   return check_launch("token_loss_join");
@@ -769,7 +828,7 @@ int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
 
 size_t rows_workspace(int T, int V, int n_top) {
   if (T <= 0 || V <= kRowCols) return 0;
-  const int part = part_len(T, V, n_top > 0), n = (V + part - 1) / part;
+  const int part = part_len(T, V), n = (V + part - 1) / part;
   return n > 1 ? (size_t)T * n * (sizeof(float4) + n_top * sizeof(u64)) : 0;
 }
 
