@@ -84,14 +84,25 @@ struct Sums {
   float m, s, su;
 };
 
-template <class X>
-__device__ __forceinline__ void finish_logprobs(const RowArgs& a, const X* row, int64_t t, const Sums& r) {
-  const int64_t tok = a.tokens[t];
+// A row's token and its logit, asked for before the row is summed.
+struct Token {
+  int64_t tok;
+  float x;
+  Token() = default;
+  template <class X>
+  __device__ __forceinline__ Token(const RowArgs& a, const X* row, int64_t t) {
+    tok = a.tokens[t];
+    x = tok >= 0 && tok < a.V ? Row<X>::one(row, tok) : 0.0f;
+  }
+};
+
+__device__ __forceinline__ void finish_logprobs(const RowArgs& a, const Token& k, int64_t t, const Sums& r) {
+  const int64_t tok = k.tok;
   const float log_s = logf(r.s);
   const bool empty = r.s == 0.0f;  // no column above -inf
   float lp = 0.0f;
   if (tok >= a.V) lp = __builtin_nanf("");
-  else if (tok >= 0) lp = empty ? -INFINITY : (Row<X>::one(row, tok) - r.m) * a.inv_t - log_s;
+  else if (tok >= 0) lp = empty ? -INFINITY : (k.x - r.m) * a.inv_t - log_s;
   a.logprob[t] = lp;
   a.entropy[t] = empty ? 0.0f : log_s - r.su * kLn2 / r.s;
   if (a.stats) {
@@ -101,9 +112,9 @@ __device__ __forceinline__ void finish_logprobs(const RowArgs& a, const X* row, 
 }
 
 __device__ __forceinline__ void put_top(const RowArgs& a, int64_t t, int rank, u64 key, const Sums& r) {
-  a.top_ids[t * a.n_top + rank] = (int32_t)~(uint32_t)key;
-  a.top_lp[t * a.n_top + rank] =
-      r.s == 0.0f ? -INFINITY : (key_value((uint32_t)(key >> 32)) - r.m) * a.inv_t - logf(r.s);
+  const float x = key_value((uint32_t)(key >> 32));
+  a.top_ids[t * a.n_top + rank] = (int)~(uint32_t)key;
+  a.top_lp[t * a.n_top + rank] = r.s == 0.0f ? -INFINITY : (x - r.m) * a.inv_t - logf(r.s);
 }
 
 // The divergence of row t by one wave, from the sums of the columns not listed (rest.m = -inf: none).
@@ -210,33 +221,41 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   }
 }
 
-// Rank of every candidate among the n in LDS (two places past them are written) by counting the larger keys,
-// two candidates a pass; those of rank below `want` go to put(rank, key).
-template <int NT, class P>
-__device__ __forceinline__ void rank_keys(u64* cand, int n, int want, int tid, P put) {
+// Ranks of the candidates: n words {value bits, column} of LDS become keys in place (room for two more), and each
+// counts the larger ones, two candidates a pass; those of rank below `want` go to put(rank, key).
+__device__ __forceinline__ u64 raw_cand(float x, int col) { return (u64)__float_as_uint(x) << 32 | (uint32_t)~col; }
+
+template <int NT, class S, class P>
+__device__ __forceinline__ void rank_cands(u64* cand, int n, int want, int tid, S sync, P put) {
+  for (int c = tid; c < n + 2; c += NT) {
+    const u64 raw = cand[c];
+    cand[c] = c < n ? (u64)value_key(__uint_as_float((uint32_t)(raw >> 32))) << 32 | (uint32_t)raw : 0;
+  }
+  sync();
   for (int c = tid; c < n; c += 2 * NT) {
-    const u64 mine[2] = {cand[c], c + NT < n ? cand[c + NT] : ~0ull};
-    int rank[2] = {0, 0};
+    const u64 k0 = cand[c], k1 = c + NT < n ? cand[c + NT] : ~0ull;
+    int r0 = 0, r1 = 0;
+#pragma unroll 2
     for (int j = 0; j < n; j += 2) {
       const u64 x = cand[j], y = cand[j + 1];
-      rank[0] += (x > mine[0]) + (y > mine[0]);
-      rank[1] += (x > mine[1]) + (y > mine[1]);
+      r0 += (x > k0) + (y > k0);
+      r1 += (x > k1) + (y > k1);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (c + i * NT < n && rank[i] < want) put(rank[i], mine[i]);
+    if (r0 < want) put(r0, k0);
+    if (c + NT < n && r1 < want) put(r1, k1);
   }
 }
 
-// The want-th largest of 256 keys (four per lane), to its leading bits above bit `low`: at least `want` keys are
-// not below the result.
+// The want-th largest of 64 G keys (G per lane), to its bits from `low` up: at least `want` keys are not below
+// the result.
+template <int G>
 __device__ __forceinline__ uint32_t nth_key(const uint32_t* k, int want, int low, bool exact) {
   uint32_t thr = 0;
   for (int b = 31; b >= low; --b) {
     const uint32_t c = thr | 1u << b;
     int n = 0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) n += __popcll(__ballot(k[g] >= c));
+    for (int g = 0; g < G; ++g) n += __popcll(__ballot(k[g] >= c));
     if (n >= want) thr = c;
     if (n == want && !exact) break;
   }
@@ -256,11 +275,11 @@ __device__ __forceinline__ void wave_fence() {
 // a threshold that n columns reach at least; those that do go to LDS and each finds its rank there.  Rows whose
 // ties bring more than LDS holds find the n-th value and the last of its columns by bits.
 template <class X, int E, bool DIST, bool TOP>
-__global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
+__global__ void __launch_bounds__(256, TOP ? 6 : 8) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, NV = E / VE, COLS = 64 * VE;
   static_assert(NV * VE == E && NV >= 4 && NV % 4 == 0, "whole vectors, four groups of them");
   __shared__ uint32_t s_mask[DIST ? 4 : 1][DIST ? 2 * E : 1];
-  __shared__ u64 s_cand[TOP ? 4 : 1][TOP ? kCandWave + 2 : 1];
+  __shared__ __align__(16) u64 s_cand[TOP ? 4 : 1][TOP ? kCandWave + 2 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= a.T) return;
@@ -281,6 +300,10 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
     }
   }
 
+  [[maybe_unused]] const Token token = [&] {
+    if constexpr (DIST) return Token{};
+    else return Token(a, row, t);
+  }();
   bool unique = true;
   if constexpr (DIST) {
     uint32_t* mask = s_mask[wave];
@@ -306,21 +329,30 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
   }
 
   // maxima (a NaN column shows in the sums)
-  uint32_t gk[4];
-  float m = -INFINITY;
+  // in four groups that short rows fill too: single vectors of fp32, halves of bf16 ones
+  float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    float gm = -INFINITY;
+  for (int i = 0; i < NV; ++i) {
+    if (i * COLS >= len) continue;
 #pragma unroll
-    for (int i = g * (NV / 4); i < (g + 1) * (NV / 4); ++i)
-      if (i * COLS < len) gm = words_max<X>(w[i], gm);
-    m = fmaxf(m, gm);
-    gk[g] = value_key(gm);
+    for (int j = 0; j < VE; j += 4) {
+      float& g = gm[VE == 8 ? (i & 1) * 2 + j / 4 : i & 3];
+      g = max3(max3(g, Row<X>::get(w[i], j), Row<X>::get(w[i], j + 1)), Row<X>::get(w[i], j + 2), Row<X>::get(w[i], j + 3));
+    }
   }
+  float m = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
   m = wave_max(m);
   uint32_t thr = 0;
   const int want = a.n_top;
-  if constexpr (TOP) thr = nth_key(gk, want, VE == 8 ? 16 : 12, false);  // 16 bits are all of a bf16 value
+  if constexpr (TOP) {
+    // as few maxima as bring few columns more than asked for: 32 of 64 about 44, 64 of 128 about 89, 128 of 256 about 177
+    constexpr int kLow = VE == 8 ? 16 : 12;  // 16 bits are all of a bf16 value
+    const uint32_t g4[4] = {value_key(gm[0]), value_key(gm[1]), value_key(gm[2]), value_key(gm[3])};
+    const uint32_t g2[2] = {g4[0] > g4[2] ? g4[0] : g4[2], g4[1] > g4[3] ? g4[1] : g4[3]};
+    const uint32_t g1 = g2[0] > g2[1] ? g2[0] : g2[1];
+    thr = want <= 32 ? nth_key<1>(&g1, want, kLow, false) : want <= 64 ? nth_key<2>(g2, want, kLow, false)
+                                                                       : nth_key<4>(g4, want, kLow, false);
+  }
 
   forget(w);
   const float m0 = m == -INFINITY ? 0.0f : m;
@@ -342,7 +374,7 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
   if constexpr (DIST) {
     finish_distill(a, row, t, r, unique, lane);
   } else {
-    if (lane == 0) finish_logprobs(a, row, t, r);
+    if (lane == 0) finish_logprobs(a, token, t, r);
   }
 
   if constexpr (TOP) {
@@ -363,7 +395,7 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
           const u64 who = __ballot(here);
           if (who == 0) continue;
           const int pos = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-          if (here && pos < kCandWave) cand[pos] = full_key(x, off + j);
+          if (here && pos < kCandWave) cand[pos] = raw_cand(x, off + j);
           n += __popcll(who);
         }
       }
@@ -403,9 +435,7 @@ __global__ void __launch_bounds__(256, (E / Row<X>::VE * 4 <= 32 ? 8 : 5)) rows_
         return k > kth || (k == kth && at <= last);
       });
     }
-    if (lane < 2) cand[n + lane] = 0;
-    wave_fence();
-    rank_keys<64>(cand, n, want, lane, [&](int rank, u64 key) { put_top(a, t, rank, key, r); });
+    rank_cands<64>(cand, n, want, lane, wave_fence, [&](int rank, u64 key) { put_top(a, t, rank, key, r); });
   }
 }
 
@@ -425,9 +455,9 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   __shared__ Sums s_sums[4];
   __shared__ float s_bmax[TOP ? kStreamCols / COLS : 1][TOP ? 256 : 1];
   __shared__ uint32_t s_key[TOP ? 256 : 1];
-  __shared__ u64 s_cand[TOP ? kCandGroup + 2 : 1];
+  __shared__ __align__(16) u64 s_cand[TOP ? kCandGroup + 2 : 1];
   __shared__ int s_items[TOP ? kItems : 1];
-  __shared__ int s_ctl[4];  // items, candidates, threshold
+  __shared__ int s_ctl[2];  // items, candidates, threshold
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t = blockIdx.x / (unsigned)a.nparts;
   const int p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
@@ -445,6 +475,10 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   };
   Words next[kBatch];
   load(0, next);
+  [[maybe_unused]] const Token token = [&] {
+    if constexpr (DIST) return Token{};
+    else return Token(a, row, t);
+  }();
   bool unique = true;
   if constexpr (DIST) {
     for (int i = tid; i < (len + 31) / 32; i += 256) s_mask[i] = 0;
@@ -530,7 +564,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   }
   if (wave == 0) {
     if constexpr (TOP) {
-      const uint32_t thr = nth_key(keys, want, VE == 8 ? 16 : 12, false);
+      const uint32_t thr = nth_key<4>(keys, want, VE == 8 ? 16 : 12, false);
       if (lane == 0) s_ctl[2] = (int)thr;
     }
     if (a.nparts > 1) {
@@ -538,7 +572,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     } else if constexpr (DIST) {
       finish_distill(a, row, t, r, unique, lane);
     } else {
-      if (lane == 0) finish_logprobs(a, row, t, r);
+      if (lane == 0) finish_logprobs(a, token, t, r);
     }
   }
   if constexpr (TOP) {
@@ -546,7 +580,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     const float least = key_value((uint32_t)s_ctl[2]);  // not less than it: in (NaN and, where it is NaN, everything in)
     auto add = [&](float x, int off) {
       const int pos = atomicAdd(&s_ctl[1], 1);
-      if (pos < kCandGroup) s_cand[pos] = full_key(x, c0 + off);
+      if (pos < kCandGroup) s_cand[pos] = raw_cand(x, c0 + off);
     };
     if (!(most < least)) {
       for (int b = 0; b * COLS < len; ++b)
@@ -592,7 +626,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
         return total(c);
       };
       // the value of rank `want`: the lanes' own want-th maximum where fewer columns exceed it, else by bits above it
-      uint32_t kth = nth_key(keys, want, 0, true);
+      uint32_t kth = nth_key<4>(keys, want, 0, true);
       int over = above(kth);
       if (over >= want) {
         const uint32_t floor = kth;
@@ -641,10 +675,8 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
       __syncthreads();
       n = s_ctl[1];
     }
-    if (tid < 2) s_cand[n + tid] = 0;
-    __syncthreads();
     u64* out = a.part_keys + (t * a.nparts + p) * want;
-    rank_keys<256>(s_cand, n, want, tid, [&](int rank, u64 key) {
+    rank_cands<256>(s_cand, n, want, tid, [] { __syncthreads(); }, [&](int rank, u64 key) {
       if (a.nparts > 1) out[rank] = key;
       else put_top(a, t, rank, key, r);
     });
@@ -678,7 +710,7 @@ __global__ void __launch_bounds__(TOP ? 256 : 64) rows_join_kernel(const X* __re
   if constexpr (DIST) {
     finish_distill(a, row, t, r, false, lane);
   } else {
-    if (threadIdx.x == 0) finish_logprobs(a, row, t, r);
+    if (threadIdx.x == 0) finish_logprobs(a, Token(a, row, t), t, r);
   }
   if constexpr (TOP) {
     const int K = a.n_top, n = a.nparts * K;
