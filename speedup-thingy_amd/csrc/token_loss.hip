@@ -262,7 +262,6 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t* k, int want, int low
   return thr;
 }
 
-constexpr int kRowCols = 2048;  // columns of a row that one wave holds
 constexpr int kCandWave = 512, kCandGroup = 1024;
 
 __device__ __forceinline__ void wave_fence() {
@@ -275,7 +274,7 @@ __device__ __forceinline__ void wave_fence() {
 // a threshold that n columns reach at least; those that do go to LDS and each finds its rank there.  Rows whose
 // ties bring more than LDS holds find the n-th value and the last of its columns by bits.
 template <class X, int E, bool DIST, bool TOP>
-__global__ void __launch_bounds__(256, TOP ? 6 : 8) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
+__global__ void __launch_bounds__(256, E / Row<X>::VE * 4 > 16 ? (TOP ? 5 : 8) : TOP ? 7 : 8) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, NV = E / VE, COLS = 64 * VE;
   static_assert(NV * VE == E && NV >= 4 && NV % 4 == 0, "whole vectors, four groups of them");
   __shared__ uint32_t s_mask[DIST ? 4 : 1][DIST ? 2 * E : 1];
@@ -829,8 +828,13 @@ __global__ void __launch_bounds__(256)
     if (here[i]) Row<X>::put(out, col[i], gt * cf[i]);
 }
 
-// Ranges of a row of more than kRowCols columns: a workgroup takes up to kStreamCols, and rows too few to give
-// every CU two workgroups are cut further, down to 8192 columns.
+// Rows that one wave holds in 32 registers or fewer, where there are four waves of them for every CU; a row of its
+// own workgroup otherwise.  (65536 rows, 20 alternatives, wave / workgroup in us: bf16 x 4096 208 / 290, x 3000
+// 177 / 271, fp32 x 4096, 64 registers, 319 / 310; one bf16 row of 3000 8.8 / 6.3.)
+bool by_wave(int T, int V, bool f32) { return T >= 1024 && V <= (f32 ? 2048 : 4096); }
+
+// Ranges of a row: a workgroup takes up to kStreamCols columns, and rows too few to give every CU two workgroups
+// are cut further, down to 8192 columns.
 int part_len(int T, int V) {
   const int least = (V + kStreamCols - 1) / kStreamCols, most = (V + 8191) / 8192;
   const int wanted = (512 + T - 1) / T;
@@ -841,8 +845,12 @@ int part_len(int T, int V) {
 template <class X, bool DIST, bool TOP>
 int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
   const X* x = static_cast<const X*>(logits);
-  if (a.V <= kRowCols) {
-    hipLaunchKernelGGL((rows_wave_kernel<X, kRowCols / 64, DIST, TOP>), dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
+  if (by_wave(a.T, a.V, Row<X>::VE == 4)) {
+    auto fn = rows_wave_kernel<X, 32, DIST, TOP>;
+    if constexpr (Row<X>::VE == 8) {
+      if (a.V > 2048) fn = rows_wave_kernel<X, 64, DIST, TOP>;
+    }
+    hipLaunchKernelGGL(fn, dim3((a.T + 3) / 4), dim3(256), 0, s, x, a);
     return check_launch("token_loss_rows");
   }
   a.part = part_len(a.T, a.V);
@@ -859,7 +867,7 @@ int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
 }
 
 size_t rows_workspace(int T, int V, int n_top) {
-  if (T <= 0 || V <= kRowCols) return 0;
+  if (T <= 0) return 0;
   const int part = part_len(T, V), n = (V + part - 1) / part;
   return n > 1 ? (size_t)T * n * (sizeof(float4) + n_top * sizeof(u64)) : 0;
 }

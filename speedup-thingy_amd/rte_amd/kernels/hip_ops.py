@@ -1466,22 +1466,23 @@ class PoolBalanceFn(torch.autograd.Function):
     def forward(ctx, logits, ids, mask):
         dev = logits.device
         C, k = logits.shape[-1], ids.shape[-1]
+        T = ids.numel() // k
         lg, ld = _logit_rows(logits)
-        T = lg.shape[0]
-        ic = _ids32(ids.reshape(T, k))
-        mc = None if mask is None else mask.reshape(T).contiguous().view(torch.uint8)
+        ic = _ids32(ids)
+        mc = None if mask is None else mask.contiguous()  # bytes of 0 and 1
         out = torch.empty((2,), dtype=F32, device=dev)
         counts = torch.empty((C,), dtype=torch.int32, device=dev)
         frac = torch.empty((C + 1,), dtype=F32, device=dev)
         with _on_device(dev):
-            ws = _scratch(_lib.load().rte_pool_balance_workspace_bytes(T, C), dev)
+            wsn = _lib.load().rte_pool_balance_workspace_bytes(T, C)
+            ws = _scratch(wsn, dev)
             call("rte_pool_balance_fwd", ptr(lg), ld, int(lg.dtype == F32), T, C, ptr(ic), k, ptr(mc), ptr(out),
-                 ptr(counts), ptr(frac), ptr(ws), ws.numel(), _s())
+                 ptr(counts), ptr(frac), ptr(ws), wsn, _s())
         ctx.save_for_backward(lg, mc, frac)
-        ctx.meta = (logits.shape, T, C, ld)
+        ctx.meta = (logits.shape, T, ld)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
-        return out[0], out[1], counts
+        return (*out.unbind(0), counts)
 
     @staticmethod
     @once_differentiable
@@ -1489,14 +1490,12 @@ class PoolBalanceFn(torch.autograd.Function):
         if g_bal is None and g_z is None:
             return None, None, None
         lg, mc, frac = ctx.saved_tensors
-        shape, T, C, ld = ctx.meta
-        gb = None if g_bal is None else g_bal.reshape(1).contiguous().to(F32)
-        gz = None if g_z is None else g_z.reshape(1).contiguous().to(F32)
-        dx = torch.empty((T, C), dtype=lg.dtype, device=lg.device)
-        with _on_device(lg.device):
-            call("rte_pool_balance_bwd", ptr(lg), ld, int(lg.dtype == F32), T, C, ptr(mc), ptr(frac), ptr(gb), ptr(gz),
-                 ptr(dx), _s())
-        return dx.view(shape), None, None
+        shape, T, ld = ctx.meta
+        gb, gz = _row_grad(g_bal), _row_grad(g_z)
+        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
+        call("rte_pool_balance_bwd", ptr(lg), ld, int(lg.dtype == F32), T, shape[-1], ptr(mc), ptr(frac), ptr(gb), ptr(gz),
+             ptr(dx), _s())
+        return dx, None, None
 
 
 def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -1607,8 +1606,10 @@ MAX_TOP = 128  # alternatives per row, of token_logprobs and topk_distill
 
 
 def _logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """x [..., V] as [T, V] rows with contiguous columns (a view where its strides allow) and their stride."""
+    """x [..., V] as rows with contiguous columns (a view where its strides allow) and their stride."""
     V = x.shape[-1]
+    if x.is_contiguous():
+        return x, V
     x2 = x.detach().reshape(-1, V)
     if x2.stride(1) != 1 and V > 1:
         x2 = x2.contiguous()
@@ -1626,9 +1627,14 @@ def _on_device(dev: torch.device):
     return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
-    """A call's own workspace (the allocator keeps those of a captured call with its graph)."""
-    return torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+def _scratch(nbytes: int, dev: torch.device):
+    """A call's own workspace, None for none (the allocator keeps those of a captured call with its graph)."""
+    return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _dense(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """t contiguous in dtype, itself where it is."""
+    return t if t.dtype == dtype and t.is_contiguous() else t.contiguous().to(dtype)
 
 
 def _whole_numbers(op: str, t: torch.Tensor) -> None:
@@ -1638,9 +1644,7 @@ def _whole_numbers(op: str, t: torch.Tensor) -> None:
 
 def _ids32(t: torch.Tensor) -> torch.Tensor:
     """t contiguous in 32 bits; wider numbers that do not fit stay out of every range."""
-    if t.dtype == torch.int64:
-        t = t.clamp(-1, 0x7FFFFFFF)
-    return t.contiguous().to(torch.int32)
+    return _dense(t.clamp(-1, 0x7FFFFFFF) if t.dtype == torch.int64 else t, torch.int32)
 
 
 def _temperature(op: str, t: float) -> float:
@@ -1661,8 +1665,34 @@ def _aligned16(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _row_grad(g, T: int):
-    return None if g is None else g.reshape(T).contiguous().to(F32)
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def _row_grad(g):
+    """An upstream gradient for a kernel.  (Backward passes launch as they are: autograd has made the tensors'
+    device and the forward's stream the current ones.)"""
+    return None if g is None else _dense(g, F32)
+
+
+def _token_logprobs(logits, tokens, n_top: int, temperature: float, need: bool):
+    """(results, what the backward needs or None) of rte_token_logprobs_fwd."""
+    dev = logits.device
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    T = tokens.numel()
+    lg, ld = _logit_rows(logits)
+    tk = _dense(tokens, torch.int64)
+    lp = torch.empty(lead, dtype=F32, device=dev)
+    ent = torch.empty(lead, dtype=F32, device=dev)
+    top_lp = torch.empty((*lead, n_top), dtype=F32, device=dev)
+    top_ids = torch.empty((*lead, n_top), dtype=torch.int32, device=dev)
+    stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
+    with _on_device(dev):
+        wsn = _lib.load().rte_token_logprobs_workspace_bytes(T, V, n_top)
+        ws = _scratch(wsn, dev)
+        call("rte_token_logprobs_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, n_top, ptr(lp),
+             ptr(ent), ptr(top_lp), ptr(top_ids), ptr(stats), ptr(ws), wsn, _s())
+    return (lp, ent, top_lp, top_ids), (lg, ld, tk, stats) if need else None
 
 
 class TokenLogprobsFn(torch.autograd.Function):
@@ -1671,27 +1701,12 @@ class TokenLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, n_top: int, temperature: float):
-        dev = logits.device
-        lead, V = logits.shape[:-1], logits.shape[-1]
-        lg, ld = _logit_rows(logits)
-        T = lg.shape[0]
-        tk = tokens.reshape(T).contiguous().to(torch.int64)
-        lp = torch.empty((T,), dtype=F32, device=dev)
-        ent = torch.empty((T,), dtype=F32, device=dev)
-        top_lp = torch.empty((T, n_top), dtype=F32, device=dev)
-        top_ids = torch.empty((T, n_top), dtype=torch.int32, device=dev)
-        need = ctx.needs_input_grad[0]
-        stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
-        with _on_device(dev):
-            ws = _scratch(_lib.load().rte_token_logprobs_workspace_bytes(T, V, n_top), dev)
-            call("rte_token_logprobs_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, n_top,
-                 ptr(lp), ptr(ent), ptr(top_lp), ptr(top_ids), ptr(stats), ptr(ws), ws.numel(), _s())
-        if need:
-            ctx.save_for_backward(lg, tk, stats, ent)
-            ctx.meta = (logits.shape, ld, temperature)
-        ctx.mark_non_differentiable(top_lp, top_ids)
+        out, (lg, ld, tk, stats) = _token_logprobs(logits, tokens, n_top, temperature, True)
+        ctx.save_for_backward(lg, tk, stats, out[1])
+        ctx.meta = (logits.shape, ld, temperature)
+        ctx.mark_non_differentiable(*out[2:])
         ctx.set_materialize_grads(False)
-        return lp.view(lead), ent.view(lead), top_lp.view(*lead, n_top), top_ids.view(*lead, n_top)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -1700,13 +1715,11 @@ class TokenLogprobsFn(torch.autograd.Function):
             return None, None, None, None
         lg, tk, stats, ent = ctx.saved_tensors
         shape, ld, temperature = ctx.meta
-        T, V = lg.shape
-        gl, ge = _row_grad(g_lp, T), _row_grad(g_ent, T)
-        dx = torch.empty((T, V), dtype=lg.dtype, device=lg.device)
-        with _on_device(lg.device):
-            call("rte_token_logprobs_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, ptr(stats),
-                 ptr(ent), ptr(gl), ptr(ge), ptr(dx), _s())
-        return dx.view(shape), None, None, None
+        gl, ge = _row_grad(g_lp), _row_grad(g_ent)
+        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
+        call("rte_token_logprobs_bwd", ptr(lg), ld, int(lg.dtype == F32), tk.numel(), shape[-1], ptr(tk), temperature,
+             ptr(stats), ptr(ent), ptr(gl), ptr(ge), ptr(dx), _s())
+        return dx, None, None, None
 
 
 def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
@@ -1726,7 +1739,10 @@ def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
         raise ValueError(f"token_logprobs: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     if not 0 <= int(n_top) <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: n_top must be in [0, min({MAX_TOP}, V)], got {n_top}")
-    return TokenLogprobsFn.apply(logits, tokens, int(n_top), _temperature("token_logprobs", temperature))
+    t = _temperature("token_logprobs", temperature)
+    if not _wants_grad(logits):
+        return _token_logprobs(logits, tokens, int(n_top), t, False)[0]
+    return TokenLogprobsFn.apply(logits, tokens, int(n_top), t)
 
 
 class LMHeadLogprobsFn(torch.autograd.Function):
@@ -1748,22 +1764,24 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         V = wb.shape[0]
         dev = hb.device
         lib = _lib.load()
-        tk = tokens.reshape(T).contiguous().to(torch.int64)
+        tk = _dense(tokens, torch.int64).view(T)
         lp = torch.empty((T,), dtype=F32, device=dev)
         ent = torch.empty((T,), dtype=F32, device=dev)
         stats = torch.empty((T, 2), dtype=F32, device=dev)
         with _on_device(dev):
             if lib.rte_lm_head_logprobs_ok(T, d, V):
-                ws = _scratch(lib.rte_lm_head_logprobs_workspace_bytes(T, V), dev)
+                wsn = lib.rte_lm_head_logprobs_workspace_bytes(T, V)
+                ws = _scratch(wsn, dev)
                 call("rte_lm_head_logprobs_fwd", ptr(hb), ptr(wb), T, d, V, ptr(tk), temperature, ptr(lp), ptr(ent),
-                     ptr(stats), ptr(ws), ws.numel(), _s())
+                     ptr(stats), ptr(ws), wsn, _s())
             else:
                 for lo in range(0, T, LMHeadLogprobsFn.ROWS):
                     hi = min(T, lo + LMHeadLogprobsFn.ROWS)
                     logits = gemm(hb[lo:hi], wb, out_f32=True)
-                    ws = _scratch(lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0), dev)
+                    wsn = lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0)
+                    ws = _scratch(wsn, dev)
                     call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0,
-                         ptr(lp[lo:]), ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), ws.numel(), _s())
+                         ptr(lp[lo:]), ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), wsn, _s())
         ctx.save_for_backward(hb, wb, tk, stats, ent)
         ctx.meta = (shape, hidden.dtype, w.dtype, temperature)
         ctx.set_materialize_grads(False)
@@ -1778,14 +1796,13 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         shape, h_dt, w_dt, temperature = ctx.meta
         T, V = hb.shape[0], wb.shape[0]
         need_h, need_w = ctx.needs_input_grad[:2]
-        gl, ge = _row_grad(g_lp, T), _row_grad(g_ent, T)
+        gl, ge = (None if g is None else _row_grad(g).view(T) for g in (g_lp, g_ent))
         if T == 0:
             dh, dw = hb.new_zeros(hb.shape), wb.new_zeros(wb.shape)
         else:
             fused = _lib.load().rte_lm_head_logprobs_ok(T, hb.shape[1], V)
             grads = LMHeadLogprobsFn._grads if fused else LMHeadLogprobsFn._grads_by_rows
-            with _on_device(hb.device):
-                dh, dw = grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_dt == BF16)
+            dh, dw = grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_dt == BF16)
         return dh.view(shape).to(h_dt) if need_h else None, dw.to(w_dt) if need_w else None, None, None
 
     @staticmethod
@@ -1861,31 +1878,36 @@ def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[to
     return LMHeadLogprobsFn.apply(hidden, w, tokens, t)
 
 
+def _topk_distill(logits, ids, teacher, temperature: float, tail: bool, need: bool):
+    """(loss, what the backward needs or None) of rte_topk_distill_fwd."""
+    dev = logits.device
+    lead, V, K = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
+    T = ids.numel() // K
+    lg, ld = _logit_rows(logits)
+    ic = _ids32(ids)
+    tc = _dense(teacher, F32)
+    loss = torch.empty(lead, dtype=F32, device=dev)
+    stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
+    cols = torch.empty((T, K), dtype=torch.int32, device=dev) if need else None
+    coef = torch.empty((T, K), dtype=F32, device=dev) if need else None
+    with _on_device(dev):
+        wsn = _lib.load().rte_topk_distill_workspace_bytes(T, V, K)
+        ws = _scratch(wsn, dev)
+        call("rte_topk_distill_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), K, temperature, int(tail),
+             ptr(loss), ptr(stats), ptr(cols), ptr(coef), ptr(ws), wsn, _s())
+    return loss, (lg, ld, stats, cols, coef) if need else None
+
+
 class TopkDistillFn(torch.autograd.Function):
     """Divergence of rows of logits from a teacher's listed columns (rte_topk_distill_*)."""
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, temperature: float, tail: bool):
-        dev = logits.device
-        lead, V, K = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
-        lg, ld = _logit_rows(logits)
-        T = lg.shape[0]
-        ic = _ids32(ids.reshape(T, K))
-        tc = teacher.detach().reshape(T, K).contiguous().to(F32)
-        loss = torch.empty((T,), dtype=F32, device=dev)
-        need = ctx.needs_input_grad[0]
-        stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
-        cols = torch.empty((T, K), dtype=torch.int32, device=dev) if need else None
-        coef = torch.empty((T, K), dtype=F32, device=dev) if need else None
-        with _on_device(dev):
-            ws = _scratch(_lib.load().rte_topk_distill_workspace_bytes(T, V, K), dev)
-            call("rte_topk_distill_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), K, temperature,
-                 int(tail), ptr(loss), ptr(stats), ptr(cols), ptr(coef), ptr(ws), ws.numel(), _s())
-        if need:
-            ctx.save_for_backward(lg, stats, cols, coef)
-            ctx.meta = (logits.shape, ld, temperature)
+        loss, (lg, ld, stats, cols, coef) = _topk_distill(logits, ids, teacher, temperature, tail, True)
+        ctx.save_for_backward(lg, stats, cols, coef)
+        ctx.meta = (logits.shape, ld, temperature)
         ctx.set_materialize_grads(False)
-        return loss.view(lead)
+        return loss
 
     @staticmethod
     @once_differentiable
@@ -1894,13 +1916,12 @@ class TopkDistillFn(torch.autograd.Function):
             return (None,) * 5
         lg, stats, cols, coef = ctx.saved_tensors
         shape, ld, temperature = ctx.meta
-        T, V = lg.shape
-        gc = _row_grad(g, T)
-        dx = torch.empty((T, V), dtype=lg.dtype, device=lg.device)
-        with _on_device(lg.device):
-            call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, V, cols.shape[1], temperature,
-                 ptr(stats), ptr(cols), ptr(coef), ptr(gc), ptr(dx), _s())
-        return dx.view(shape), None, None, None, None
+        T, K = cols.shape
+        gc = _row_grad(g)
+        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
+        call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, shape[-1], K, temperature, ptr(stats),
+             ptr(cols), ptr(coef), ptr(gc), ptr(dx), _s())
+        return dx, None, None, None, None
 
 
 def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False) -> torch.Tensor:
@@ -1926,7 +1947,10 @@ def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.
                          f"logits {tuple(logits.shape)}")
     if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
         raise ValueError(f"topk_distill: lists of 1 to {MAX_TOP} entries expected, got {teacher_ids.shape[-1]}")
-    return TopkDistillFn.apply(logits, teacher_ids, teacher_logits, _temperature("topk_distill", temperature), bool(tail))
+    t = _temperature("topk_distill", temperature)
+    if not _wants_grad(logits):
+        return _topk_distill(logits, teacher_ids, teacher_logits.detach(), t, bool(tail), False)[0]
+    return TopkDistillFn.apply(logits, teacher_ids, teacher_logits.detach(), t, bool(tail))
 
 
 # ----------------------------------------------------------------------------- audit distillation
