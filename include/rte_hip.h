@@ -644,19 +644,20 @@ int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V
  *      in the reference; beside rte_gemm_bf16 + rte_ce_fwd) ----
  * hidden bf16 [T, d], w bf16 [V, d], logits = hidden w^T (fp32 accumulation); _ok: sizes the tile product
  * takes (d a multiple of 64 from 128, operands below 2 GiB).  fwd: logprob, entropy as
- * rte_token_logprobs_fwd (an infinite logit makes its row NaN), stats f32 [T] for the backward.  dlogits: the gradient of logits columns col0 .. col0 + n in bf16 [T, n]
- * (n % 8 == 0), computed from the product again with w_rows = those n rows of w (rows past V are the
- * caller's to fill up, with zeros say): the caller multiplies it with w_rows and hidden. */
+ * rte_token_logprobs_fwd (an infinite logit makes its row NaN), stats f32 [T] for the backward.
+ * bwd: dhidden bf16 [T, d] and dw [V, d] (f32 or bf16), NULL = not wanted, for g_logprob / g_entropy f32 [T]
+ * (NULL = 0).  The logits are computed again, their gradient in bf16 for `width` (a multiple of 64) tokens of
+ * the vocabulary at a time: 2 T width bytes of the workspace. */
 int rte_lm_head_logprobs_ok(int T, int d, int V);
 size_t rte_lm_head_logprobs_workspace_bytes(int T, int V);
 int rte_lm_head_logprobs_fwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
                              float temperature, float* logprob, float* entropy, float* stats, void* workspace,
                              size_t workspace_bytes, void* stream);
-size_t rte_lm_head_dlogits_workspace_bytes(int T);
-int rte_lm_head_dlogits(const void* hidden, const void* w_rows, int T, int d, int V, int col0, int n,
-                        const int64_t* tokens, float temperature, const float* stats, const float* entropy,
-                        const float* g_logprob, const float* g_entropy, void* dlogits, void* workspace,
-                        size_t workspace_bytes, void* stream);
+size_t rte_lm_head_logprobs_bwd_workspace_bytes(int T, int d, int V, int width, int need_dh, int need_dw);
+int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
+                             float temperature, const float* stats, const float* entropy, const float* g_logprob,
+                             const float* g_entropy, int width, void* dhidden, void* dw, int dw_f32, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ---- divergence from a teacher's top logits (no counterpart in the reference, whose
  *      macro_distill_loss needs the teacher's whole row) ----

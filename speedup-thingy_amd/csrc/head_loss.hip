@@ -12,6 +12,8 @@
 
 namespace rte {
 
+int cast_f32_bf16(const float* x, int64_t n, bf16* y, hipStream_t s);
+
 namespace {
 
 constexpr int kRows = 16, kSlices = 16;  // of a join workgroup: sixteen rows' blocks are read 256 bytes at a time
@@ -90,6 +92,68 @@ int tiles(const void* w, const void* h, int n, int T, int d, const Epilogue& e, 
   return gemm_tile_launch(p, kind, s, 1, nullptr, 0, &splits);
 }
 
+// Rows lo .. lo + n of w [V, d] with zeros past V (their logits' gradients add nothing to dh).
+__global__ void head_pad_kernel(const bf16* __restrict__ w, int lo, int V, int64_t d, int64_t n, bf16* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n * d) out[i] = lo + i / d < V ? w[lo * d + i] : 0;
+}
+
+__global__ void head_rows_out_kernel(const float* __restrict__ x, int64_t n, int f32, void* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  if (f32) static_cast<float*>(out)[i] = x[i];
+  else static_cast<bf16*>(out)[i] = f2bf(x[i]);
+}
+
+// out [M, N] (+)= the product of two operands given as in memory, on the library's dense GEMM.
+int product(const void* a, int64_t lda, int a_t, const void* b, int64_t ldb, int b_t, void* out, int f32, int M, int N, int K,
+            float beta, void* ws, size_t ws_bytes, hipStream_t s) {
+  GemmArgs p;
+  p.a.ptr = static_cast<const bf16*>(a);
+  p.a.ld = lda;
+  p.b.ptr = static_cast<const bf16*>(b);
+  p.b.ld = ldb;
+  p.a_t = a_t, p.b_t = b_t;
+  p.M = M, p.N = N, p.K = K;
+  p.epi.c = out;
+  p.epi.ldc = N;
+  p.epi.c_f32 = f32;
+  p.epi.beta = beta;
+  return gemm_launch(p, EPI_STORE, s, ws, ws_bytes);
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+// The backward's vocabulary ranges: `width` columns each (a multiple of 64) over the whole 64s, then the rest.
+struct Ranges {
+  int width, whole, rest, rest8;
+  Ranges(int V, int w) : width(w), whole(V / 64 * 64), rest(V % 64), rest8((V % 64 + 7) / 8 * 8) {
+    if (width > whole) width = whole;
+  }
+  int most() const { return width > rest8 ? width : rest8; }
+  bool one() const { return whole == 0 || (rest == 0 && width == whole); }
+};
+
+struct BwdSpace {
+  size_t rows, grad, dh, pad, tail, gemm, total;
+  BwdSpace(int T, int d, int V, const Ranges& r, bool h, bool w) {
+    rows = 0;
+    grad = up((size_t)T * sizeof(float4));
+    dh = grad + up((size_t)T * r.most() * sizeof(bf16));
+    pad = dh + (h && !r.one() ? up((size_t)T * d * sizeof(float)) : 0);
+    const bool ragged = r.rest8 != r.rest;
+    tail = pad + (ragged ? up((size_t)r.rest8 * d * sizeof(bf16)) : 0);
+    gemm = tail + (ragged && w ? up((size_t)r.rest8 * d * sizeof(float)) : 0);
+    size_t g = 0;
+    for (int n : {r.width, r.whole ? (r.whole - 1) % (r.width ? r.width : 1) + 1 : 0, r.rest8}) {
+      if (n <= 0) continue;
+      if (h && gemm_splitk_bytes(T, d, n) > g) g = gemm_splitk_bytes(T, d, n);
+      if (w && gemm_splitk_bytes(n, d, T) > g) g = gemm_splitk_bytes(n, d, T);
+    }
+    total = gemm + up(g);
+  }
+};
+
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -130,32 +194,74 @@ int rte_lm_head_logprobs_fwd(const void* hidden, const void* w, int T, int d, in
   return check_launch("lm_head_logprobs_join");
 }
 
-size_t rte_lm_head_dlogits_workspace_bytes(int T) { return T > 0 ? (size_t)T * sizeof(float4) : 0; }
+size_t rte_lm_head_logprobs_bwd_workspace_bytes(int T, int d, int V, int width, int need_dh, int need_dw) {
+  if (!rte_lm_head_logprobs_ok(T, d, V) || width < 64 || width % 64 != 0) return 0;
+  return BwdSpace(T, d, V, Ranges(V, width), need_dh, need_dw).total;
+}
 
-int rte_lm_head_dlogits(const void* hidden, const void* w_rows, int T, int d, int V, int col0, int n, const int64_t* tokens,
-                        float temperature, const float* stats, const float* entropy, const float* g_logprob,
-                        const float* g_entropy, void* dlogits, void* ws, size_t ws_bytes, void* stream) {
-  RTE_REQUIRE(rte_lm_head_logprobs_ok(T, d, V), "lm_head_dlogits: size not taken (T %d, d %d, V %d)", T, d, V);
-  RTE_REQUIRE(n >= 8 && n % 8 == 0 && col0 >= 0 && col0 < V && n - 8 < V - col0,
-              "lm_head_dlogits: need a multiple of 8 columns that starts inside V and covers it at most");
-  RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "lm_head_dlogits: temperature must be positive and finite");
-  RTE_REQUIRE(hidden && w_rows && tokens && stats && entropy && dlogits, "lm_head_dlogits: null argument");
-  RTE_REQUIRE(aligned(hidden) && aligned(w_rows) && aligned(dlogits) && aligned(ws),
-              "lm_head_dlogits: operands must be 16-byte aligned");
-  RTE_REQUIRE(ws && ws_bytes >= rte_lm_head_dlogits_workspace_bytes(T), "lm_head_dlogits: workspace too small");
+int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
+                             float temperature, const float* stats, const float* entropy, const float* g_logprob,
+                             const float* g_entropy, int width, void* dhidden, void* dw, int dw_f32, void* ws,
+                             size_t ws_bytes, void* stream) {
+  RTE_REQUIRE(rte_lm_head_logprobs_ok(T, d, V), "lm_head_logprobs_bwd: size not taken (T %d, d %d, V %d)", T, d, V);
+  RTE_REQUIRE(width >= 64 && width % 64 == 0, "lm_head_logprobs_bwd: width must be a positive multiple of 64");
+  RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "lm_head_logprobs_bwd: temperature must be positive and finite");
+  RTE_REQUIRE(hidden && w && tokens && stats && entropy, "lm_head_logprobs_bwd: null argument");
+  RTE_REQUIRE(aligned(hidden) && aligned(w) && aligned(dhidden) && aligned(dw) && aligned(ws),
+              "lm_head_logprobs_bwd: operands must be 16-byte aligned");
+  if (!dhidden && !dw) return 0;
+  const Ranges r(V, width);
+  const BwdSpace at(T, d, V, r, dhidden != nullptr, dw != nullptr);
+  RTE_REQUIRE((int64_t)T * r.most() < (int64_t)1 << 30, "lm_head_logprobs_bwd: width too large for %d rows", T);
+  RTE_REQUIRE(ws && ws_bytes >= at.total, "lm_head_logprobs_bwd: workspace too small");
   auto s = static_cast<hipStream_t>(stream);
-  Epilogue e;
-  e.c = dlogits;
-  e.ldc = n;
-  e.c2 = (float)(1.4426950408889634 / temperature);
-  e.col0 = col0;
-  e.tokens = tokens;
-  float4* rows = static_cast<float4*>(ws);
-  e.row_in = rows;
+  char* base = static_cast<char*>(ws);
+  float4* rows = reinterpret_cast<float4*>(base + at.rows);
+  void* grad = base + at.grad;
+  void* gemm_ws = base + at.gemm;
+  const size_t gemm_bytes = at.total - at.gemm;
+  float* dh32 = reinterpret_cast<float*>(base + at.dh);
   hipLaunchKernelGGL(head_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, s, T, V, tokens, stats, entropy, g_logprob,
                      g_entropy, 1.0f / temperature, rows);
   RTE_TRY(check_launch("lm_head_rows"));
-  return tiles(w_rows, hidden, n, T, d, e, EPI_DLOGITS, s);
+  for (int lo = 0; lo < V;) {
+    const bool last = lo == r.whole;  // the columns past the whole 64s
+    int n = last ? r.rest8 : r.whole - lo < r.width ? r.whole - lo : r.width;
+    const int real = last ? r.rest : n;
+    const bf16* wr = static_cast<const bf16*>(w) + (int64_t)lo * d;
+    if (n != real) {
+      bf16* pad = reinterpret_cast<bf16*>(base + at.pad);
+      hipLaunchKernelGGL(head_pad_kernel, dim3((unsigned)(((int64_t)n * d + 255) / 256)), dim3(256), 0, s,
+                         static_cast<const bf16*>(w), lo, V, (int64_t)d, (int64_t)n, pad);
+      RTE_TRY(check_launch("lm_head_pad"));
+      wr = pad;
+    }
+    Epilogue e;
+    e.c = grad;
+    e.ldc = n;
+    e.c2 = (float)(1.4426950408889634 / temperature);
+    e.col0 = lo;
+    e.tokens = tokens;
+    e.row_in = rows;
+    RTE_TRY(tiles(wr, hidden, n, T, d, e, EPI_DLOGITS, s));
+    if (dhidden)  // [T, n] [n, d]; in fp32 until the last of several ranges
+      RTE_TRY(product(grad, n, 0, wr, d, 1, r.one() ? dhidden : dh32, !r.one(), T, d, n, lo > 0 ? 1.0f : 0.0f, gemm_ws,
+                      gemm_bytes, s));
+    if (dw) {     // [n, T] [T, d]
+      void* out = static_cast<char*>(dw) + (int64_t)lo * d * (dw_f32 ? 4 : 2);
+      float* tail = reinterpret_cast<float*>(base + at.tail);
+      const bool direct = n == real;
+      RTE_TRY(product(grad, n, 1, hidden, d, 1, direct ? out : tail, direct ? dw_f32 : 1, n, d, T, 0.0f, gemm_ws, gemm_bytes,
+                      s));
+      if (!direct) {
+        const int64_t k = (int64_t)real * d;
+        hipLaunchKernelGGL(head_rows_out_kernel, dim3((unsigned)((k + 255) / 256)), dim3(256), 0, s, tail, k, dw_f32, out);
+        RTE_TRY(check_launch("lm_head_rows_out"));
+      }
+    }
+    lo += real;
+  }
+  return dhidden && !r.one() ? cast_f32_bf16(dh32, (int64_t)T * d, static_cast<bf16*>(dhidden), s) : 0;
 }
 
 }  // extern "C"

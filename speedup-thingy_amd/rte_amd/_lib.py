@@ -175,8 +175,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "rte_lm_head_logprobs_ok": (_I, [_I, _I, _I]),
     "rte_lm_head_logprobs_workspace_bytes": (_SZ, [_I, _I]),
     "rte_lm_head_logprobs_fwd": (_I, [_P, _P, _I, _I, _I, _P, _F, _P, _P, _P, _P, _SZ, _P]),
-    "rte_lm_head_dlogits_workspace_bytes": (_SZ, [_I]),
-    "rte_lm_head_dlogits": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "rte_lm_head_logprobs_bwd_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "rte_lm_head_logprobs_bwd": (_I, [_P, _P, _I, _I, _I, _P, _F, _P, _P, _P, _P, _I, _P, _P, _I, _P, _SZ, _P]),
     "rte_topk_distill_workspace_bytes": (_SZ, [_I, _I, _I]),
     "rte_topk_distill_fwd": (_I, [_P, _I64, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _P, _P, _P, _SZ, _P]),
     "rte_topk_distill_bwd": (_I, [_P, _I64, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P]),

@@ -1807,34 +1807,17 @@ class LMHeadLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def _grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_bf16):
-        """Vocabulary range by vocabulary range: the gradient of its logits in bf16, then dW's rows of that
-        range and the range's part of dh (fp32 until the last).  Whole 64s of columns first: the tile product
-        of dh takes those."""
         lib = _lib.load()
         T, d = hb.shape
         V = wb.shape[0]
         dev = hb.device
-        width = max(64, LMHeadLogprobsFn.GRAD // (2 * T) // 64 * 64)
-        whole = V // 64 * 64
-        cuts = [*range(0, whole, width), whole] if whole else [0]
-        if whole < V:
-            cuts.append(V)
-        dh = torch.empty((T, d), dtype=BF16 if len(cuts) == 2 else F32, device=dev) if need_h else None
+        width = max(64, min(V, LMHeadLogprobsFn.GRAD // (2 * T)) // 64 * 64)
+        dh = torch.empty_like(hb) if need_h else None
         dw = torch.empty((V, d), dtype=BF16 if w_bf16 else F32, device=dev) if need_w else None
-        ws = _scratch(lib.rte_lm_head_dlogits_workspace_bytes(T), dev)
-        for lo, hi in zip(cuts, cuts[1:]):
-            wr, n = wb[lo:hi], (hi - lo + 7) // 8 * 8
-            if n > hi - lo:  # rows of zeros, whose gradients add nothing to dh and are dropped from dW
-                wr = torch.nn.functional.pad(wr, (0, 0, 0, n - (hi - lo)))
-            dl = torch.empty((T, n), dtype=BF16, device=dev)
-            call("rte_lm_head_dlogits", ptr(hb), ptr(wr), T, d, V, lo, n, ptr(tk), temperature, ptr(stats), ptr(ent),
-                 ptr(gl), ptr(ge), ptr(dl), ptr(ws), ws.numel(), _s())
-            if need_h:
-                gemm(dl, wr, b_t=True, out=dh, beta=float(lo > 0))
-            if need_w and n == hi - lo:
-                gemm(dl, hb, a_t=True, b_t=True, out=dw[lo:hi])
-            elif need_w:
-                dw[lo:hi] = gemm(dl, hb, a_t=True, b_t=True, out_f32=True)[: hi - lo]
+        wsn = lib.rte_lm_head_logprobs_bwd_workspace_bytes(T, d, V, width, need_h, need_w)
+        ws = _scratch(wsn, dev)
+        call("rte_lm_head_logprobs_bwd", ptr(hb), ptr(wb), T, d, V, ptr(tk), temperature, ptr(stats), ptr(ent), ptr(gl),
+             ptr(ge), width, ptr(dh), ptr(dw), int(not w_bf16), ptr(ws), wsn, _s())
         return dh, dw
 
     @staticmethod

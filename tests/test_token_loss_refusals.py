@@ -47,13 +47,18 @@ def test_lm_head_logprobs(lib):
 
     fwd(d=100), fwd(T=0), fwd(V=0), fwd(t=0.0), fwd(t=float("nan")), fwd(h=None), fwd(w=None), fwd(tok=None), fwd(lp=None)
     fwd(ent=None), fwd(st=None), fwd(ws=None), fwd(wsn=need - 1), fwd(h=BUF + 2), fwd(w=BUF + 8)
-    room = lib.rte_lm_head_dlogits_workspace_bytes(100)
+    size = lib.rte_lm_head_logprobs_bwd_workspace_bytes
+    room = size(100, 128, 1000, 256, 1, 1)
+    assert room > 2 * 100 * 256 and size(100, 128, 1000, 100, 1, 1) == 0 and size(100, 100, 1000, 256, 1, 1) == 0
 
-    def bwd(h=BUF, w=BUF, T=100, d=128, V=1000, c=0, n=64, tok=BUF, t=1.0, st=BUF, ent=BUF, dl=BUF, ws=BUF, wsn=room):
-        refused(lib, "rte_lm_head_dlogits", h, w, T, d, V, c, n, tok, t, st, ent, BUF, BUF, dl, ws, wsn, None)
+    def bwd(h=BUF, w=BUF, T=100, d=128, V=1000, tok=BUF, t=1.0, st=BUF, ent=BUF, width=256, dh=BUF, dw=BUF, ws=BUF, wsn=room):
+        refused(lib, "rte_lm_head_logprobs_bwd", h, w, T, d, V, tok, t, st, ent, BUF, BUF, width, dh, dw, 0, ws, wsn, None)
 
-    bwd(c=-8), bwd(c=1000), bwd(c=936, n=72), bwd(n=0), bwd(n=60), bwd(n=1008), bwd(d=100), bwd(t=-1.0), bwd(st=None), bwd(ent=None)
-    bwd(dl=None), bwd(dl=BUF + 4), bwd(ws=None), bwd(wsn=room - 1), bwd(tok=None), bwd(h=None), bwd(w=None)
+    bwd(width=0), bwd(width=100), bwd(d=100), bwd(t=-1.0), bwd(st=None), bwd(ent=None), bwd(dh=BUF + 2), bwd(dw=BUF + 4)
+    bwd(ws=None), bwd(wsn=room - 1), bwd(tok=None), bwd(h=None), bwd(w=None), bwd(T=0)
+    bwd(T=1 << 22, V=1 << 20, width=1 << 20, wsn=1 << 50)
+    assert lib.rte_lm_head_logprobs_bwd(BUF, BUF, 100, 128, 1000, BUF, 1.0, BUF, BUF, None, None, 64, None, None, 0, None, 0,
+                                        None) == 0  # nothing wanted
 
 
 def test_topk_distill(lib):
