@@ -78,11 +78,11 @@ struct Epilogue {
   int S = 0, H = 0, hd = 0, dmodel = 0;
   // log probabilities: the product is taken as w h^T, m counts the vocabulary (col0 first), n the rows of h
   float c2 = 0.0f;                   // log2(e) / temperature
-  int col0 = 0;
+  int col0 = 0, cols = 0;            // EPI_DLOGITS: rows m from cols on are fill, their gradient 0
   const int64_t* tokens = nullptr;   // [N]
   float4* row_part = nullptr;        // EPI_ROW_SUMS: [gemm_tile_row_blocks, N] {max, sum 2^u, sum 2^u u, -}, u in log2
   float* tok_logit = nullptr;        // EPI_ROW_SUMS: [N], written where the token is one of the columns
-  const float4* row_in = nullptr;    // EPI_DLOGITS: [N] {log2 of the normaliser, a, b, g / t}: d = 2^lp (a + b lp)
+  const float4* row_in = nullptr;    // EPI_DLOGITS: [N] {max, a, b, g / t}: d = 2^u (a + b u), u = x c2 - max
 };
 
 struct GemmArgs {

@@ -235,6 +235,13 @@ __device__ __forceinline__ void dlogits64(const Epilogue& e, const f32x16_v (&ac
       *reinterpret_cast<uint2*>(patch + l32 * 128 + (((4 * i + q) ^ (l32 & 7)) << 4) + half * 8) =
           make_uint2(pack_bf2(d[0], d[1]), pack_bf2(d[2], d[3]));
     }
+  if (m0 + 64 > e.cols) {  // a fill row's logit, 0, may be far above every real one
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const int v = (k >> 2) * 8 + 4 * half + (k & 3);
+      if (m0 + v >= e.cols) *reinterpret_cast<bf16*>(patch + l32 * 128 + (((v >> 3) ^ (l32 & 7)) << 4) + (v & 7) * 2) = 0;
+    }
+  }
   const int64_t rel = n < N && row.w != 0.0f ? e.tokens[n] - e.col0 - m0 : -1;
   const bool hit = rel >= 0 && rel < 64 && ((rel >> 2) & 1) == half;
   wave_lds_fence();

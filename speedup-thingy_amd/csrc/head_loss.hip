@@ -63,11 +63,13 @@ __global__ void __launch_bounds__(kRows* kSlices)
                : empty   ? -INFINITY
                          : (__builtin_fmaf(tok_logit[t], c2, -a.m) - log_s) * kLn2;
   entropy[t] = empty ? 0.0f : (log_s - a.su / a.s) * kLn2;
-  stats[t] = a.m + log_s;
+  stats[2 * t] = a.m;
+  stats[2 * t + 1] = log_s;
 }
 
-// What the backward's epilogue needs of a row: with l = log2 p, dx_v = p_v (a + b l) + [v = token] g / t,
-// a = -(g + g_H entropy) / t, b = -g_H ln 2 / t.
+// What the backward's epilogue needs of a row.  With l = log2 of e^{(x_v - m) / t}, m as rounded in the sums, and S
+// their total: p_v = 2^l / S and dx_v = 2^l (a + b l) + [v = token] g / t, where
+// b = -g_H ln 2 / (t S), a = -(g + g_H entropy) / (t S) - b log2 S.
 __global__ void head_rows_kernel(int T, int V, const int64_t* __restrict__ tokens, const float* __restrict__ stats,
                                  const float* __restrict__ entropy, const float* __restrict__ g_lp,
                                  const float* __restrict__ g_ent, float inv_t, float4* __restrict__ rows) {
@@ -75,7 +77,8 @@ __global__ void head_rows_kernel(int T, int V, const int64_t* __restrict__ token
   if (t >= T) return;
   const int64_t tok = tokens[t];
   const float g = g_lp && tok >= 0 && tok < V ? g_lp[t] * inv_t : 0.0f, gh = g_ent ? g_ent[t] * inv_t : 0.0f;
-  rows[t] = make_float4(stats[t], -(g + gh * entropy[t]), -gh * kLn2, g);
+  const float log_s = stats[2 * t + 1], inv_s = exp2_(-log_s), b = -gh * kLn2 * inv_s;
+  rows[t] = make_float4(stats[2 * t], -(g + gh * entropy[t]) * inv_s - b * log_s, b, g);
 }
 
 // The product w h^T over n rows of w on the tile kernels.
@@ -241,6 +244,7 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
     e.ldc = n;
     e.c2 = (float)(1.4426950408889634 / temperature);
     e.col0 = lo;
+    e.cols = real;
     e.tokens = tokens;
     e.row_in = rows;
     RTE_TRY(tiles(wr, hidden, n, T, d, e, EPI_DLOGITS, s));

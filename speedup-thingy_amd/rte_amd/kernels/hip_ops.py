@@ -262,12 +262,14 @@ def gemm(
     out: torch.Tensor | None = None,
     beta: float = 0.0,
     b_rows: torch.Tensor | None = None,
+    own_ws: bool = False,
 ) -> torch.Tensor:
     """C[m, n] = alpha * sum_k A(m, k) B(n, k) (+ beta C) (+ resid).
 
     a: [M, K] (a_t False) or [K, M] (a_t True); b: [N, K] (b_t False) or [K, N] (b_t True).
     b_rows (int32, optional): B's memory rows are b_rows[n] (b_t False) or b_rows[k] (b_t True),
     so b may hold more rows than the problem reads.  bf16 operands, fp32 accumulation.
+    own_ws: a workspace of this call's own instead of the stream's cached one.
     """
     _lib.require_device_tensors("gemm", a, b, resid, out, b_rows)
     if a.dtype != BF16 or b.dtype != BF16:
@@ -290,7 +292,12 @@ def gemm(
         out = torch.empty((M, N), dtype=F32 if out_f32 else BF16, device=a.device)
     if resid is not None:
         resid = resid.contiguous().to(F32)
-    wsp, wsn = _gemm_ws(M, N, K, a.device)
+    if own_ws:
+        wsn = _lib.load().rte_gemm_workspace_bytes(M, N, K)
+        ws = _scratch(wsn, a.device)
+        wsp = ptr(ws)
+    else:
+        wsp, wsn = _gemm_ws(M, N, K, a.device)
     call(
         "rte_gemm_bf16",
         ptr(a), a.shape[1], int(a_t), None,
@@ -1750,7 +1757,7 @@ class LMHeadLogprobsFn(torch.autograd.Function):
 
     Where the tile product takes the sizes (rte_lm_head_logprobs_ok) the logits stay in its accumulators;
     the backward multiplies again, GRAD bytes of logit gradients at a time.  Other widths go through
-    fp32 logits of ROWS tokens at a time."""
+    fp32 logits of ROWS tokens at a time.  Workspaces are the call's own: a captured call keeps its."""
 
     ROWS = 2048
     GRAD = 1 << 30
@@ -1777,7 +1784,7 @@ class LMHeadLogprobsFn(torch.autograd.Function):
             else:
                 for lo in range(0, T, LMHeadLogprobsFn.ROWS):
                     hi = min(T, lo + LMHeadLogprobsFn.ROWS)
-                    logits = gemm(hb[lo:hi], wb, out_f32=True)
+                    logits = gemm(hb[lo:hi], wb, out_f32=True, own_ws=True)
                     wsn = lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0)
                     ws = _scratch(wsn, dev)
                     call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0,
@@ -1828,7 +1835,7 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
         for lo in range(0, T, LMHeadLogprobsFn.ROWS):
             hi = min(T, lo + LMHeadLogprobsFn.ROWS)
-            logits = gemm(hb[lo:hi], wb, out_f32=True)
+            logits = gemm(hb[lo:hi], wb, out_f32=True, own_ws=True)
             dl = torch.empty_like(logits)
             call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
                  ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(dl), _s())
@@ -1836,9 +1843,9 @@ class LMHeadLogprobsFn(torch.autograd.Function):
             if V % 8:
                 dl = torch.nn.functional.pad(dl, (0, -V % 8))
             if need_h:
-                gemm(dl, wp, b_t=True, out=dh[lo:hi])
+                gemm(dl, wp, b_t=True, out=dh[lo:hi], own_ws=True)
             if need_w:
-                dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True)[:V]
+                dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True, own_ws=True)[:V]
         return dh, dw
 
 

@@ -117,7 +117,7 @@ def test_nothing_left(H):
         ids = torch.zeros(x.shape[0], 2, dtype=torch.int32, device=DEV)
         bal, z, counts = H.pool_balance(leaf, ids, mask=mask)
         (dx,) = torch.autograd.grad(bal + z, leaf)
-        assert float(bal) == 0 and float(z) == 0 and not counts.any() and not dx.any() and dx.shape == x.shape
+        assert float(bal.detach()) == 0 and float(z.detach()) == 0 and not counts.any() and not dx.any() and dx.shape == x.shape
 
 
 def test_nan_is_seen(H):
