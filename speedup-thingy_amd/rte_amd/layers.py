@@ -104,7 +104,12 @@ class ClusterPoolSwiGLU(nn.Module):
     """Routed cluster-pool SwiGLU: d_ff neurons in `ffn_clusters` contiguous pools, each token
     routed to its top-`ffn_top_k` pools by logits x @ Wr^T, pool outputs combined with softmax
     weights over the selected logits.  Dense parameters (wug, wd) stay the source of truth as in
-    StaticClusterPoolSwiGLU (rte/layers.py:119-220)."""
+    StaticClusterPoolSwiGLU (rte/layers.py:119-220).
+
+    Given a list as `balance_into`, each forward appends the routing's (balance loss, router z-loss, counts
+    [ffn_clusters]) to it, for a training program to weigh into its loss (the routing itself gives the router no
+    gradient towards pools a token was not sent to).  The entries hold their graph: the program empties the list
+    once it has its loss, before it captures a backward pass of the same parameters in any case."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
@@ -116,13 +121,26 @@ class ClusterPoolSwiGLU(nn.Module):
         self.wd = nn.Linear(config.d_ff, d, bias=False)
         self.last_ids: torch.Tensor | None = None
         self.last_weights: torch.Tensor | None = None
+        self.balance_into: list[tuple[torch.Tensor, torch.Tensor, torch.Tensor]] | None = None
 
     def forward(self, x: torch.Tensor, resid: torch.Tensor | None = None) -> torch.Tensor:
         out, ids, w = hip_ops.routed_cluster_pool_swiglu(
             x, self.router.weight, self.wug.weight, self.wd.weight, self.top_k, resid=resid
         )
         self.last_ids, self.last_weights = ids, w
+        if self.balance_into is not None:
+            self.balance_into.append(self.balance(x, ids))
         return out
+
+    def balance(self, x: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None = None):
+        """hip_ops.pool_balance of the router's logits on x [..., d], whose tokens were sent to the pools ids
+        ([tokens, k]); mask (bool [...]) leaves tokens out."""
+        w = self.router.weight
+        pad = -w.shape[0] % 8  # the GEMM's backward reads 8 logits at a time
+        if pad:
+            w = torch.cat([w, w.new_zeros(pad, w.shape[1])])
+        logits = hip_ops.linear(x, w, out_f32=True)[..., : self.n_clusters]
+        return hip_ops.pool_balance(logits, ids.view(*x.shape[:-1], ids.shape[-1]), mask=mask)
 
 
 class PackedDenseSwiGLU(nn.Module):
