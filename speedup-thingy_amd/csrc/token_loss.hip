@@ -111,10 +111,10 @@ __device__ __forceinline__ void finish_logprobs(const RowArgs& a, const Token& k
   }
 }
 
-__device__ __forceinline__ void put_top(const RowArgs& a, int64_t t, int rank, u64 key, const Sums& r) {
+__device__ __forceinline__ void put_top(const RowArgs& a, int64_t t, int rank, u64 key, const Sums& r, float log_s) {
   const float x = key_value((uint32_t)(key >> 32));
   a.top_ids[t * a.n_top + rank] = (int)~(uint32_t)key;
-  a.top_lp[t * a.n_top + rank] = r.s == 0.0f ? -INFINITY : (x - r.m) * a.inv_t - logf(r.s);
+  a.top_lp[t * a.n_top + rank] = r.s == 0.0f ? -INFINITY : (x - r.m) * a.inv_t - log_s;
 }
 
 // The divergence of row t by one wave, from the sums of the columns not listed (rest.m = -inf: none).
@@ -221,29 +221,92 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   }
 }
 
-// Ranks of the candidates: n words {value bits, column} of LDS become keys in place (room for two more), and each
-// counts the larger ones, two candidates a pass; those of rank below `want` go to put(rank, key).
-__device__ __forceinline__ u64 raw_cand(float x, int col) { return (u64)__float_as_uint(x) << 32 | (uint32_t)~col; }
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
-template <int NT, class S, class P>
-__device__ __forceinline__ void rank_cands(u64* cand, int n, int want, int tid, S sync, P put) {
-  for (int c = tid; c < n + 2; c += NT) {
-    const u64 raw = cand[c];
-    cand[c] = c < n ? (u64)value_key(__uint_as_float((uint32_t)(raw >> 32))) << 32 | (uint32_t)raw : 0;
-  }
-  sync();
-  for (int c = tid; c < n; c += 2 * NT) {
-    const u64 k0 = cand[c], k1 = c + NT < n ? cand[c + NT] : ~0ull;
-    int r0 = 0, r1 = 0;
-#pragma unroll 2
-    for (int j = 0; j < n; j += 2) {
-      const u64 x = cand[j], y = cand[j + 1];
-      r0 += (x > k0) + (y > k0);
-      r1 += (x > k1) + (y > k1);
+// Candidates: {value bits, column} words of LDS as they are found, keys once they are all there.
+__device__ __forceinline__ u64 raw_cand(float x, int col) { return (u64)__float_as_uint(x) << 32 | (uint32_t)~col; }
+__device__ __forceinline__ u64 cand_key(u64 raw) {
+  return (u64)value_key(__uint_as_float((uint32_t)(raw >> 32))) << 32 | (uint32_t)raw;
+}
+
+// v of the lane whose number differs in the bit O.
+template <int O>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  const int x = (int)v;
+  if constexpr (O == 1) return __builtin_amdgcn_update_dpp(x, x, 0xb1, 0xf, 0xf, false);
+  else if constexpr (O == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4e, 0xf, 0xf, false);
+  else if constexpr (O == 4) {  // 7 - lane, then 3 - lane
+    const int y = __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false);
+    return __builtin_amdgcn_update_dpp(y, y, 0x1b, 0xf, 0xf, false);
+  } else if constexpr (O == 8) return __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false);  // a rotation by half a row
+  else return __shfl_xor(v, O, 64);
+}
+
+// Bitonic sort, largest first, of 64 R keys that lie R to a lane (key lane R + r): K the length of the runs being
+// merged, J the distance compared.
+template <int R, int K, int J>
+__device__ __forceinline__ void sort_step(u64 (&v)[R], int lane) {
+  if constexpr (J >= R) {
+    const bool first = ((lane & (K / R)) == 0) == ((lane & (J / R)) == 0);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const u64 o = (u64)lane_xor<J / R>((uint32_t)(v[r] >> 32)) << 32 | lane_xor<J / R>((uint32_t)v[r]);
+      v[r] = (v[r] > o) == first ? v[r] : o;
     }
-    if (r0 < want) put(r0, k0);
-    if (c + NT < n && r1 < want) put(r1, k1);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r & J) continue;
+      const bool down = K < R ? (r & K) == 0 : (lane & (K / R)) == 0;
+      const u64 a = v[r], b = v[r | J];
+      const bool keep = (a > b) == down;
+      v[r] = keep ? a : b;
+      v[r | J] = keep ? b : a;
+    }
   }
+  if constexpr (J > 1) sort_step<R, K, J / 2>(v, lane);
+}
+template <int R, int K = 2>
+__device__ __forceinline__ void sort_keys(u64 (&v)[R], int lane) {
+  sort_step<R, K, K / 2>(v, lane);
+  if constexpr (K < 64 * R) sort_keys<R, K * 2>(v, lane);
+}
+
+// One wave sorts the n candidates in its registers and hands the first `want` to put(rank, key); ranks past the
+// last candidate get key 0.
+template <int R, class P>
+__device__ __forceinline__ void sort_cands(const u64* cand, int n, int want, int lane, P put) {
+  u64 v[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = r * 64 + lane < n ? cand_key(cand[r * 64 + lane]) : 0;
+  sort_keys<R>(v, lane);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane * R + r < want) put(lane * R + r, v[r]);
+}
+
+// The same for any n by one wave: from 17 to 256 sorted; few, or more (rows with many ties at the threshold),
+// ranked by counting the larger keys.  (All ranked by counting, 8192 rows of 2048 fp32 took 32 us for 64
+// alternatives and 51 for 128; 28 and 35 sorted.)
+template <class P>
+__device__ __forceinline__ void order_cands(u64* cand, int n, int want, int lane, P put) {
+  if (n > 16) {
+    if (n <= 64 && want <= 64) return sort_cands<1>(cand, n, want, lane, put);
+    if (n <= 128) return sort_cands<2>(cand, n, want, lane, put);
+    if (n <= 256) return sort_cands<4>(cand, n, want, lane, put);
+  }
+  for (int c = lane; c < n; c += 64) cand[c] = cand_key(cand[c]);
+  wave_fence();
+  for (int c = lane; c < n; c += 64) {
+    const u64 mine = cand[c];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += cand[j] > mine;
+    if (rank < want) put(rank, mine);
+  }
+  for (int c = n + lane; c < want; c += 64) put(c, 0ull);
 }
 
 // The want-th largest of 64 G keys (G per lane), to its bits from `low` up: at least `want` keys are not below
@@ -264,21 +327,16 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t* k, int want, int low
 
 constexpr int kCandWave = 512, kCandGroup = 1024;
 
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // A short row by one wave, held in registers: E columns per lane, read once.  The maximum comes first, so no
 // sum is rescaled.  For the alternatives, the n-th largest of 256 maxima (of quarters of the lanes' columns) is
 // a threshold that n columns reach at least; those that do go to LDS and each finds its rank there.  Rows whose
 // ties bring more than LDS holds find the n-th value and the last of its columns by bits.
 template <class X, int E, bool DIST, bool TOP>
-__global__ void __launch_bounds__(256, E / Row<X>::VE * 4 > 16 ? (TOP ? 5 : 8) : TOP ? 7 : 8) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
+__global__ void __launch_bounds__(256, TOP ? (E == 64 ? 4 : 6) : 8) rows_wave_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, NV = E / VE, COLS = 64 * VE;
   static_assert(NV * VE == E && NV >= 4 && NV % 4 == 0, "whole vectors, four groups of them");
   __shared__ uint32_t s_mask[DIST ? 4 : 1][DIST ? 2 * E : 1];
-  __shared__ __align__(16) u64 s_cand[TOP ? 4 : 1][TOP ? kCandWave + 2 : 1];
+  __shared__ __align__(16) u64 s_cand[TOP ? 4 : 1][TOP ? kCandWave : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= a.T) return;
@@ -434,7 +492,8 @@ __global__ void __launch_bounds__(256, E / Row<X>::VE * 4 > 16 ? (TOP ? 5 : 8) :
         return k > kth || (k == kth && at <= last);
       });
     }
-    rank_cands<64>(cand, n, want, lane, wave_fence, [&](int rank, u64 key) { put_top(a, t, rank, key, r); });
+    const float log_s = logf(s);
+    order_cands(cand, n, want, lane, [&](int rank, u64 key) { put_top(a, t, rank, key, r, log_s); });
   }
 }
 
@@ -454,7 +513,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   __shared__ Sums s_sums[4];
   __shared__ float s_bmax[TOP ? kStreamCols / COLS : 1][TOP ? 256 : 1];
   __shared__ uint32_t s_key[TOP ? 256 : 1];
-  __shared__ __align__(16) u64 s_cand[TOP ? kCandGroup + 2 : 1];
+  __shared__ __align__(16) u64 s_cand[TOP ? kCandGroup : 1];
   __shared__ int s_items[TOP ? kItems : 1];
   __shared__ int s_ctl[2];  // items, candidates, threshold
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -674,13 +733,13 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
       __syncthreads();
       n = s_ctl[1];
     }
+    if (wave != 0) return;
     u64* out = a.part_keys + (t * a.nparts + p) * want;
-    rank_cands<256>(s_cand, n, want, tid, [] { __syncthreads(); }, [&](int rank, u64 key) {
+    const float log_s = logf(r.s);
+    order_cands(s_cand, n, want, lane, [&](int rank, u64 key) {
       if (a.nparts > 1) out[rank] = key;
-      else put_top(a, t, rank, key, r);
+      else put_top(a, t, rank, key, r, log_s);
     });
-    if (a.nparts > 1)  // a short last range
-      for (int c = n + tid; c < want; c += 256) out[c] = 0;
   }
 }
 
@@ -715,6 +774,7 @@ __global__ void __launch_bounds__(TOP ? 256 : 64) rows_join_kernel(const X* __re
     const int K = a.n_top, n = a.nparts * K;
     const u64* keys = a.part_keys + t * n;
     const bool fits = n <= kJoinKeys;
+    const float log_s = logf(r.s);
     if (fits) {
       for (int i = threadIdx.x; i < n; i += 256) s_keys[i] = keys[i];
       __syncthreads();
@@ -733,7 +793,7 @@ __global__ void __launch_bounds__(TOP ? 256 : 64) rows_join_kernel(const X* __re
         }
         rank += lo;
       }
-      if (rank < K) put_top(a, t, rank, mine, r);
+      if (rank < K) put_top(a, t, rank, mine, r, log_s);
     }
   }
 }
