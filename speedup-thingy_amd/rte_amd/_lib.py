@@ -14,6 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "librte_hip.so"
+OPS_PATH = LIB_PATH.with_name("librte_ops.so")  # autograd nodes in C++ over librte_hip (torch.ops.rte)
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -219,6 +220,22 @@ def load() -> ctypes.CDLL:
         fn.argtypes = args
     _LIB = lib
     return lib
+
+
+_OPS = None
+
+
+def ops():
+    """torch.ops.rte: the token losses and the pool balance with their gradients (csrc/loss_ops.cpp); raises if
+    the library is not built."""
+    global _OPS
+    if _OPS is None:
+        load()
+        if not OPS_PATH.exists():
+            raise RuntimeError(f"{OPS_PATH} is not built; run speedup-thingy_amd/build.py")
+        torch.ops.load_library(str(OPS_PATH))
+        _OPS = torch.ops.rte
+    return _OPS
 
 
 def loaded() -> bool:

@@ -1466,45 +1466,6 @@ def router_aux(probs, expected_depth, usage_ema, *, coverage_min: float, lambda_
     return {"load": load, "cover": cover, "depth": depth}
 
 
-class PoolBalanceFn(torch.autograd.Function):
-    """Balance loss, router z-loss and counts of routed pools (rte_pool_balance_*)."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, mask):
-        dev = logits.device
-        C, k = logits.shape[-1], ids.shape[-1]
-        T = ids.numel() // k
-        lg, ld = _logit_rows(logits)
-        ic = _ids32(ids)
-        mc = None if mask is None else mask.contiguous()  # bytes of 0 and 1
-        out = torch.empty((2,), dtype=F32, device=dev)
-        counts = torch.empty((C,), dtype=torch.int32, device=dev)
-        frac = torch.empty((C + 1,), dtype=F32, device=dev)
-        with _on_device(dev):
-            wsn = _lib.load().rte_pool_balance_workspace_bytes(T, C)
-            ws = _scratch(wsn, dev)
-            call("rte_pool_balance_fwd", ptr(lg), ld, int(lg.dtype == F32), T, C, ptr(ic), k, ptr(mc), ptr(out),
-                 ptr(counts), ptr(frac), ptr(ws), wsn, _s())
-        ctx.save_for_backward(lg, mc, frac)
-        ctx.meta = (logits.shape, T, ld)
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        return (*out.unbind(0), counts)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_bal, g_z, _g_counts):
-        if g_bal is None and g_z is None:
-            return None, None, None
-        lg, mc, frac = ctx.saved_tensors
-        shape, T, ld = ctx.meta
-        gb, gz = _row_grad(g_bal), _row_grad(g_z)
-        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
-        call("rte_pool_balance_bwd", ptr(lg), ld, int(lg.dtype == F32), T, shape[-1], ptr(mc), ptr(frac), ptr(gb), ptr(gz),
-             ptr(dx), _s())
-        return dx, None, None
-
-
 def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(balance, z, counts int32 [C]) of router logits [..., C] (float32 or bfloat16, C <= 1024) whose rows
     were sent to the pools ids [..., k] (route_topk's; outside [0, C): none).
@@ -1526,7 +1487,7 @@ def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor,
         raise ValueError("pool_balance: fewer than 2^31 (row, pool) pairs expected")
     if mask is not None and (mask.dtype != torch.bool or mask.shape != lead):
         raise ValueError(f"pool_balance: mask must be bool {tuple(lead)}, got {mask.dtype} {tuple(mask.shape)}")
-    return PoolBalanceFn.apply(logits, ids, mask)
+    return _lib.ops().pool_balance(logits, ids, mask, _lib.stream_ptr(logits.device))
 
 
 # ----------------------------------------------------------------------------- LM head + cross-entropy
@@ -1612,17 +1573,6 @@ def select_logit_rows(logits: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
 MAX_TOP = 128  # alternatives per row, of token_logprobs and topk_distill
 
 
-def _logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """x [..., V] as rows with contiguous columns (a view where its strides allow) and their stride."""
-    V = x.shape[-1]
-    if x.is_contiguous():
-        return x, V
-    x2 = x.detach().reshape(-1, V)
-    if x2.stride(1) != 1 and V > 1:
-        x2 = x2.contiguous()
-    return x2, x2.stride(0)
-
-
 def _same_device(op: str, *tensors) -> None:
     ts = [t for t in tensors if t is not None]
     if any(t.device != ts[0].device for t in ts):
@@ -1649,11 +1599,6 @@ def _whole_numbers(op: str, t: torch.Tensor) -> None:
         raise TypeError(f"{op}: whole numbers expected, got {t.dtype}")
 
 
-def _ids32(t: torch.Tensor) -> torch.Tensor:
-    """t contiguous in 32 bits; wider numbers that do not fit stay out of every range."""
-    return _dense(t.clamp(-1, 0x7FFFFFFF) if t.dtype == torch.int64 else t, torch.int32)
-
-
 def _temperature(op: str, t: float) -> float:
     t = float(t)
     if not 1e-6 <= t <= 1e6:
@@ -1670,63 +1615,6 @@ def _check_logits(op: str, logits: torch.Tensor) -> None:
 def _aligned16(t: torch.Tensor) -> torch.Tensor:
     """t, copied where it starts inside a 16-byte word."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-
-
-def _row_grad(g):
-    """An upstream gradient for a kernel.  (Backward passes launch as they are: autograd has made the tensors'
-    device and the forward's stream the current ones.)"""
-    return None if g is None else _dense(g, F32)
-
-
-def _token_logprobs(logits, tokens, n_top: int, temperature: float, need: bool):
-    """(results, what the backward needs or None) of rte_token_logprobs_fwd."""
-    dev = logits.device
-    lead, V = logits.shape[:-1], logits.shape[-1]
-    T = tokens.numel()
-    lg, ld = _logit_rows(logits)
-    tk = _dense(tokens, torch.int64)
-    lp = torch.empty(lead, dtype=F32, device=dev)
-    ent = torch.empty(lead, dtype=F32, device=dev)
-    top_lp = torch.empty((*lead, n_top), dtype=F32, device=dev)
-    top_ids = torch.empty((*lead, n_top), dtype=torch.int32, device=dev)
-    stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
-    with _on_device(dev):
-        wsn = _lib.load().rte_token_logprobs_workspace_bytes(T, V, n_top)
-        ws = _scratch(wsn, dev)
-        call("rte_token_logprobs_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(tk), temperature, n_top, ptr(lp),
-             ptr(ent), ptr(top_lp), ptr(top_ids), ptr(stats), ptr(ws), wsn, _s())
-    return (lp, ent, top_lp, top_ids), (lg, ld, tk, stats) if need else None
-
-
-class TokenLogprobsFn(torch.autograd.Function):
-    """Per row of logits: the token's log probability, the entropy and the top alternatives
-    (rte_token_logprobs_*); the backward is one pass from the saved row statistics."""
-
-    @staticmethod
-    def forward(ctx, logits, tokens, n_top: int, temperature: float):
-        out, (lg, ld, tk, stats) = _token_logprobs(logits, tokens, n_top, temperature, True)
-        ctx.save_for_backward(lg, tk, stats, out[1])
-        ctx.meta = (logits.shape, ld, temperature)
-        ctx.mark_non_differentiable(*out[2:])
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, _g_top, _g_ids):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        lg, tk, stats, ent = ctx.saved_tensors
-        shape, ld, temperature = ctx.meta
-        gl, ge = _row_grad(g_lp), _row_grad(g_ent)
-        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
-        call("rte_token_logprobs_bwd", ptr(lg), ld, int(lg.dtype == F32), tk.numel(), shape[-1], ptr(tk), temperature,
-             ptr(stats), ptr(ent), ptr(gl), ptr(ge), ptr(dx), _s())
-        return dx, None, None, None
 
 
 def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
@@ -1747,28 +1635,23 @@ def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
     if not 0 <= int(n_top) <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: n_top must be in [0, min({MAX_TOP}, V)], got {n_top}")
     t = _temperature("token_logprobs", temperature)
-    if not _wants_grad(logits):
-        return _token_logprobs(logits, tokens, int(n_top), t, False)[0]
-    return TokenLogprobsFn.apply(logits, tokens, int(n_top), t)
+    return _lib.ops().token_logprobs(logits, tokens, int(n_top), t, _lib.stream_ptr(logits.device))
 
 
 class LMHeadLogprobsFn(torch.autograd.Function):
-    """token_logprobs' first two results of hidden @ W^T without keeping the logits.
+    """token_logprobs' first two results of hb @ wb^T (bf16) over fp32 logits of ROWS tokens at a time, for the
+    sizes that the tile product does not take (rte_lm_head_logprobs_ok).  hidden and w carry the graph; the
+    products' workspaces are the call's own, so a captured call keeps them.
 
-    Where the tile product takes the sizes (rte_lm_head_logprobs_ok) the logits stay in its accumulators;
-    the backward multiplies again, GRAD bytes of logit gradients at a time.  Other widths go through
-    fp32 logits of ROWS tokens at a time.  Workspaces are the call's own: a captured call keeps its."""
+    Where the tile product takes the sizes, the logits stay in its accumulators and the backward multiplies
+    again, GRAD bytes of logit gradients at a time (rte_lm_head_logprobs_*)."""
 
     ROWS = 2048
     GRAD = 1 << 30
 
     @staticmethod
-    def forward(ctx, hidden, w, tokens, temperature: float):
-        shape = hidden.shape
-        hb = _aligned16(hidden.reshape(-1, shape[-1]).contiguous().to(BF16))
-        wb = _aligned16(cast_bf16(w))
-        T, d = hb.shape
-        V = wb.shape[0]
+    def forward(ctx, hidden, w, hb, wb, tokens, temperature: float):
+        T, V = hb.shape[0], wb.shape[0]
         dev = hb.device
         lib = _lib.load()
         tk = _dense(tokens, torch.int64).view(T)
@@ -1776,60 +1659,28 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         ent = torch.empty((T,), dtype=F32, device=dev)
         stats = torch.empty((T, 2), dtype=F32, device=dev)
         with _on_device(dev):
-            if lib.rte_lm_head_logprobs_ok(T, d, V):
-                wsn = lib.rte_lm_head_logprobs_workspace_bytes(T, V)
+            for lo in range(0, T, LMHeadLogprobsFn.ROWS):
+                hi = min(T, lo + LMHeadLogprobsFn.ROWS)
+                logits = gemm(hb[lo:hi], wb, out_f32=True, own_ws=True)
+                wsn = lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0)
                 ws = _scratch(wsn, dev)
-                call("rte_lm_head_logprobs_fwd", ptr(hb), ptr(wb), T, d, V, ptr(tk), temperature, ptr(lp), ptr(ent),
-                     ptr(stats), ptr(ws), wsn, _s())
-            else:
-                for lo in range(0, T, LMHeadLogprobsFn.ROWS):
-                    hi = min(T, lo + LMHeadLogprobsFn.ROWS)
-                    logits = gemm(hb[lo:hi], wb, out_f32=True, own_ws=True)
-                    wsn = lib.rte_token_logprobs_workspace_bytes(hi - lo, V, 0)
-                    ws = _scratch(wsn, dev)
-                    call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0,
-                         ptr(lp[lo:]), ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), wsn, _s())
+                call("rte_token_logprobs_fwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, 0, ptr(lp[lo:]),
+                     ptr(ent[lo:]), None, None, ptr(stats[lo:]), ptr(ws), wsn, _s())
         ctx.save_for_backward(hb, wb, tk, stats, ent)
-        ctx.meta = (shape, hidden.dtype, w.dtype, temperature)
+        ctx.meta = (hidden.shape, hidden.dtype, w.dtype, temperature)
         ctx.set_materialize_grads(False)
-        return lp.view(shape[:-1]), ent.view(shape[:-1])
+        return lp.view(tokens.shape), ent.view(tokens.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_ent):
         if g_lp is None and g_ent is None:
-            return None, None, None, None
+            return (None,) * 6
         hb, wb, tk, stats, ent = ctx.saved_tensors
         shape, h_dt, w_dt, temperature = ctx.meta
         T, V = hb.shape[0], wb.shape[0]
         need_h, need_w = ctx.needs_input_grad[:2]
-        gl, ge = (None if g is None else _row_grad(g).view(T) for g in (g_lp, g_ent))
-        if T == 0:
-            dh, dw = hb.new_zeros(hb.shape), wb.new_zeros(wb.shape)
-        else:
-            fused = _lib.load().rte_lm_head_logprobs_ok(T, hb.shape[1], V)
-            grads = LMHeadLogprobsFn._grads if fused else LMHeadLogprobsFn._grads_by_rows
-            dh, dw = grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_dt == BF16)
-        return dh.view(shape).to(h_dt) if need_h else None, dw.to(w_dt) if need_w else None, None, None
-
-    @staticmethod
-    def _grads(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_bf16):
-        lib = _lib.load()
-        T, d = hb.shape
-        V = wb.shape[0]
-        dev = hb.device
-        width = max(64, min(V, LMHeadLogprobsFn.GRAD // (2 * T)) // 64 * 64)
-        dh = torch.empty_like(hb) if need_h else None
-        dw = torch.empty((V, d), dtype=BF16 if w_bf16 else F32, device=dev) if need_w else None
-        wsn = lib.rte_lm_head_logprobs_bwd_workspace_bytes(T, d, V, width, need_h, need_w)
-        ws = _scratch(wsn, dev)
-        call("rte_lm_head_logprobs_bwd", ptr(hb), ptr(wb), T, d, V, ptr(tk), temperature, ptr(stats), ptr(ent), ptr(gl),
-             ptr(ge), width, ptr(dh), ptr(dw), int(not w_bf16), ptr(ws), wsn, _s())
-        return dh, dw
-
-    @staticmethod
-    def _grads_by_rows(hb, wb, tk, stats, ent, gl, ge, temperature, need_h, need_w, w_bf16):
-        T, V = hb.shape[0], wb.shape[0]
+        gl, ge = (None if g is None else _dense(g, F32).view(T) for g in (g_lp, g_ent))
         dh = torch.empty_like(hb)
         dw = torch.zeros(wb.shape, dtype=F32, device=hb.device)
         wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
@@ -1846,7 +1697,7 @@ class LMHeadLogprobsFn(torch.autograd.Function):
                 gemm(dl, wp, b_t=True, out=dh[lo:hi], own_ws=True)
             if need_w:
                 dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True, own_ws=True)[:V]
-        return dh, dw
+        return dh.view(shape).to(h_dt) if need_h else None, dw.to(w_dt) if need_w else None, None, None, None, None
 
 
 def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1865,53 +1716,13 @@ def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[to
         return token_logprobs(_f32().linear(hidden, w), tokens, temperature=t)[:2]
     if w.shape[1] % 8:
         raise ValueError(f"lm_head_logprobs: the width must be a multiple of 8, got {w.shape[1]}")
-    return LMHeadLogprobsFn.apply(hidden, w, tokens, t)
-
-
-def _topk_distill(logits, ids, teacher, temperature: float, tail: bool, need: bool):
-    """(loss, what the backward needs or None) of rte_topk_distill_fwd."""
-    dev = logits.device
-    lead, V, K = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
-    T = ids.numel() // K
-    lg, ld = _logit_rows(logits)
-    ic = _ids32(ids)
-    tc = _dense(teacher, F32)
-    loss = torch.empty(lead, dtype=F32, device=dev)
-    stats = torch.empty((T, 2), dtype=F32, device=dev) if need else None
-    cols = torch.empty((T, K), dtype=torch.int32, device=dev) if need else None
-    coef = torch.empty((T, K), dtype=F32, device=dev) if need else None
-    with _on_device(dev):
-        wsn = _lib.load().rte_topk_distill_workspace_bytes(T, V, K)
-        ws = _scratch(wsn, dev)
-        call("rte_topk_distill_fwd", ptr(lg), ld, int(lg.dtype == F32), T, V, ptr(ic), ptr(tc), K, temperature, int(tail),
-             ptr(loss), ptr(stats), ptr(cols), ptr(coef), ptr(ws), wsn, _s())
-    return loss, (lg, ld, stats, cols, coef) if need else None
-
-
-class TopkDistillFn(torch.autograd.Function):
-    """Divergence of rows of logits from a teacher's listed columns (rte_topk_distill_*)."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, temperature: float, tail: bool):
-        loss, (lg, ld, stats, cols, coef) = _topk_distill(logits, ids, teacher, temperature, tail, True)
-        ctx.save_for_backward(lg, stats, cols, coef)
-        ctx.meta = (logits.shape, ld, temperature)
-        ctx.set_materialize_grads(False)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        if g is None:
-            return (None,) * 5
-        lg, stats, cols, coef = ctx.saved_tensors
-        shape, ld, temperature = ctx.meta
-        T, K = cols.shape
-        gc = _row_grad(g)
-        dx = torch.empty(shape, dtype=lg.dtype, device=lg.device)
-        call("rte_topk_distill_bwd", ptr(lg), ld, int(lg.dtype == F32), T, shape[-1], K, temperature, ptr(stats),
-             ptr(cols), ptr(coef), ptr(gc), ptr(dx), _s())
-        return dx, None, None, None, None
+    h = hidden.detach()
+    hb = _aligned16(h.reshape(-1, h.shape[-1]).contiguous().to(BF16))
+    wb = _aligned16(cast_bf16(w).detach())
+    if _lib.load().rte_lm_head_logprobs_ok(hb.shape[0], hb.shape[1], wb.shape[0]):
+        return _lib.ops().lm_head_logprobs(hidden, w, hb, wb, tokens, t, LMHeadLogprobsFn.GRAD,
+                                           _lib.stream_ptr(hidden.device))
+    return LMHeadLogprobsFn.apply(hidden, w, hb, wb, tokens, t)
 
 
 def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False) -> torch.Tensor:
@@ -1938,9 +1749,7 @@ def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.
     if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
         raise ValueError(f"topk_distill: lists of 1 to {MAX_TOP} entries expected, got {teacher_ids.shape[-1]}")
     t = _temperature("topk_distill", temperature)
-    if not _wants_grad(logits):
-        return _topk_distill(logits, teacher_ids, teacher_logits.detach(), t, bool(tail), False)[0]
-    return TopkDistillFn.apply(logits, teacher_ids, teacher_logits.detach(), t, bool(tail))
+    return _lib.ops().topk_distill(logits, teacher_ids, teacher_logits, t, bool(tail), _lib.stream_ptr(logits.device))
 
 
 # ----------------------------------------------------------------------------- audit distillation
