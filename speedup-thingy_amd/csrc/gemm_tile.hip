@@ -164,8 +164,10 @@ __device__ __forceinline__ float swiglu_bwd8(const Epilogue& e, int m, int n, co
 
 // Log probabilities.  The product is w h^T, so a lane's accumulators hold logits of one row of h (column l32 of a
 // 32 x 32 block), rows 8 q + 4 half + 0 .. 3 of the vocabulary: a row's sums need no exchange but between the
-// two halves of the wave.  (As h w^T, through 64-column patches in LDS and three exchanges per sum, the
-// epilogue took 11 us of a 256 x 256 tile's 39; this one see the launch.)
+// two halves of the wave.  (As h w^T, through 64-column patches in LDS and three exchanges per sum, a 256 x 256
+// tile of k 1024 took 39 us; now 33.5, 26 of them products.)  8192 tokens, 32768 columns, k 1024: 537 us for the
+// sums and 558 for the gradient of the logits, where the products with that gradient take 433 and 446.  Two
+// workgroups of 256 x 128 per CU, one's output beside the other's products, took 590 and 627: half as long loads.
 template <int J, int I0, int TM, int TMA, int TN>
 __device__ __forceinline__ float find_logit(const f32x16_v (&acc)[TMA][TN], int rel, int half) {
   float x = 0.0f;
@@ -176,10 +178,12 @@ __device__ __forceinline__ float find_logit(const f32x16_v (&acc)[TMA][TN], int 
   return x;
 }
 
-// Sums of the wave's WTM vocabulary rows from m0 on for row n of h; left = vocabulary rows that exist from m0.
-template <int J, int TM, int TN>
-__device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][TN], int m0, int left, int n, int N, int half) {
-  if (left < TM * 32) {
+// Sums of the wave's WTM vocabulary rows from m0 on for row n of h and its token; left = vocabulary rows that exist
+// from m0 (ENDS: fewer than the wave's).
+template <int J, bool ENDS, int TM, int TN>
+__device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][TN], int m0, int left, int n, int N, int half,
+                                         int64_t tok) {
+  if constexpr (ENDS) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -201,12 +205,12 @@ __device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][
       const float u = __builtin_fmaf(acc[i][J][r], e.c2, -m2), w = exp2_(u);
       s += w;
       // only columns past the end are -inf among finite ones: 2^-256 is 0
-      su = __builtin_fmaf(w, left < TM * 32 ? fmaxf(u, -256.0f) : u, su);
+      su = __builtin_fmaf(w, ENDS ? fmaxf(u, -256.0f) : u, su);
     }
   s += __shfl_xor(s, 32, 64);
   su += __shfl_xor(su, 32, 64);
   if (n < N && half == 0) e.row_part[(int64_t)(m0 / (TM * 32)) * N + n] = make_float4(m2, s, su, 0.0f);
-  const int64_t rel = n < N ? e.tokens[n] - m0 : -1;
+  const int64_t rel = n < N ? tok - m0 : -1;
   const bool hit = rel >= 0 && rel < TM * 32 && rel < left && ((rel >> 2) & 1) == half;
   if (__any(hit)) {
     const float x = find_logit<J, 0, TM>(acc, (int)rel, half);
@@ -218,9 +222,8 @@ __device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][
 // that whole 128-byte lines leave.
 template <int J, int I0, int TM, int TN>
 __device__ __forceinline__ void dlogits64(const Epilogue& e, const f32x16_v (&acc)[TM][TN], int m0, int M, int nb, int N, int lane,
-                                          unsigned char* patch) {
+                                          unsigned char* patch, const float4& row, int64_t tok) {
   const int half = lane >> 5, l32 = lane & 31, n = nb + l32;
-  const float4 row = e.row_in[n < N ? n : N - 1];
   wave_lds_fence();
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -242,7 +245,7 @@ __device__ __forceinline__ void dlogits64(const Epilogue& e, const f32x16_v (&ac
       if (m0 + v >= e.cols) *reinterpret_cast<bf16*>(patch + l32 * 128 + (((v >> 3) ^ (l32 & 7)) << 4) + (v & 7) * 2) = 0;
     }
   }
-  const int64_t rel = n < N && row.w != 0.0f ? e.tokens[n] - e.col0 - m0 : -1;
+  const int64_t rel = n < N && row.w != 0.0f ? tok - e.col0 - m0 : -1;
   const bool hit = rel >= 0 && rel < 64 && ((rel >> 2) & 1) == half;
   wave_lds_fence();
   if (__any(hit)) {
@@ -525,6 +528,18 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
   }
   for (; kt + ST < nk; kt += ST)
     each_stage([&](auto s) { step(s, Young{}, std::true_type{}, kt + decltype(s)::value + ST); });
+  // what the output needs of the rows of h is on its way during the last products
+  int64_t tok[2] = {};
+  float4 row_in[2];
+  if constexpr (EPI == EPI_ROW_SUMS || EPI == EPI_DLOGITS) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      int n = n0 + wn * WTN + j * 32 + (lane & 31);
+      n = n < p.N ? n : p.N - 1;
+      tok[j] = p.epi.tokens[n];
+      if constexpr (EPI == EPI_DLOGITS) row_in[j] = p.epi.row_in[n];
+    }
+  }
   each_stage([&](auto s) {
     step(s, std::integral_constant<int, ST - 2 - decltype(s)::value>{}, std::false_type{}, 0);
   });
@@ -541,15 +556,20 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
     static_assert(TN == 2 && (TM == 2 || TM == 4), "two columns of blocks");
     const int nb = n0 + wn * WTN;
     if constexpr (EPI == EPI_ROW_SUMS) {
-      row_sums<0>(e, acc, mw, mlim - mw, nb + l32, p.N, half);
-      row_sums<1>(e, acc, mw, mlim - mw, nb + 32 + l32, p.N, half);
+      auto sums = [&](auto ends) {
+        constexpr bool E = decltype(ends)::value;
+        row_sums<0, E>(e, acc, mw, mlim - mw, nb + l32, p.N, half, tok[0]);
+        row_sums<1, E>(e, acc, mw, mlim - mw, nb + 32 + l32, p.N, half, tok[1]);
+      };
+      if (mlim - mw < WTM) sums(std::true_type{});
+      else sums(std::false_type{});
     } else {
       unsigned char* patch = reinterpret_cast<unsigned char*>(pt);
-      dlogits64<0, 0>(e, acc, mw, mlim, nb, p.N, lane, patch);
-      dlogits64<1, 0>(e, acc, mw, mlim, nb + 32, p.N, lane, patch);
+      dlogits64<0, 0>(e, acc, mw, mlim, nb, p.N, lane, patch, row_in[0], tok[0]);
+      dlogits64<1, 0>(e, acc, mw, mlim, nb + 32, p.N, lane, patch, row_in[1], tok[1]);
       if constexpr (TM == 4) {
-        dlogits64<0, 2>(e, acc, mw + 64, mlim, nb, p.N, lane, patch);
-        dlogits64<1, 2>(e, acc, mw + 64, mlim, nb + 32, p.N, lane, patch);
+        dlogits64<0, 2>(e, acc, mw + 64, mlim, nb, p.N, lane, patch, row_in[0], tok[0]);
+        dlogits64<1, 2>(e, acc, mw + 64, mlim, nb + 32, p.N, lane, patch, row_in[1], tok[1]);
       }
     }
     return;
