@@ -33,7 +33,6 @@ __device__ __forceinline__ uint32_t value_key(float x) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k > kInfKey ? 0x7fc00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
-__device__ __forceinline__ u64 full_key(float x, int col) { return (u64)value_key(x) << 32 | (uint32_t)~col; }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;  // without the canonical copies that fmaxf makes of operands it knows nothing of
@@ -521,7 +520,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
   __shared__ uint32_t s_key[TOP ? 256 : 1];
   __shared__ __align__(16) u64 s_cand[TOP ? kCandGroup : 1];
   __shared__ int s_items[TOP ? kItems : 1];
-  __shared__ int s_ctl[2];  // items, candidates, threshold
+  __shared__ int s_ctl[3];  // items, candidates, threshold
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t = blockIdx.x / (unsigned)a.nparts;
   const int p = blockIdx.x - (unsigned)t * (unsigned)a.nparts;
