@@ -212,7 +212,7 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   if (!a.stats) return;
   const bool none = foreign || !some || empty;
   if (lane == 0) {
-    const bool out = none || (rsum == 0.0 && rest.m == -INFINITY);
+    const bool out = none || rest.s == 0.0f;  // no column outside the list above -inf
     a.stats[2 * t] = out ? 0.0f : rest.m;
     // (q(R) - r) / (the rest's sum relative to its own maximum)
     a.stats[2 * t + 1] = out ? 0.0f : (float)((rsum * inv - r) / rest.s);

@@ -694,3 +694,21 @@ def test_captured(H, V):
             torch.cuda.synchronize()
             for a, b in zip(have, want):
                 assert torch.equal(a, b), f"replay {i} of {fn.__name__}"
+
+
+# ----------------------------------------------------------------------------- students limited to the list
+
+@pytest.mark.parametrize("V,repeat", [(40, 1), (3000, 1), (9001, 1), (70001, 1), (40, 256), (2000, 256)])
+def test_distill_nothing_outside_the_list(H, V, repeat):
+    """Only listed columns are possible: the others have probability 0 and gradient 0, in rows with one such column
+    and in rows with all of them."""
+    g = gen(V, 21)
+    x = torch.full((4, V), -math.inf, device=DEV)
+    ids = torch.stack([torch.randperm(V, device=DEV, generator=g)[:7] for _ in range(4)])
+    x.scatter_(1, ids, torch.randn(4, 7, device=DEV, generator=g))
+    x[1, ids[1, 1:]] = -math.inf
+    tl = torch.randn(4, 7, device=DEV, generator=g)
+    tl[1, 1:] = -math.inf
+    many = lambda v: v.repeat(repeat, 1)
+    check_distill(H, many(x), many(ids), many(tl), 1.0, False, g)
+    check_distill(H, many(x).bfloat16(), many(ids), many(tl), 2.0, False, g)
