@@ -563,7 +563,7 @@ int rte_router_aux_bwd(const float* mean_prob, const float* g_load, const float*
  * frac f32 [C + 1] = f and 1 / n, for the backward:
  *   dlogits = p (g_balance C (f - sum f p) + 2 g_z lse) / n, in the logits' type, dense [T, C]; rows
  *   without part get 0.  g_balance, g_z: device scalars, NULL = 0.
- * C <= 1024.  Two launches; sums in a fixed order. */
+ * C <= 1024, k <= 1024.  Two launches; sums in a fixed order. */
 size_t rte_pool_balance_workspace_bytes(int T, int C);
 int rte_pool_balance_fwd(const void* logits, int64_t ld, int f32, int T, int C, const int32_t* ids, int k,
                          const uint8_t* mask, float* out, int32_t* counts, float* frac, void* workspace,

@@ -362,8 +362,8 @@ size_t rte_pool_balance_workspace_bytes(int T, int C) {
 int rte_pool_balance_fwd(const void* logits, int64_t ld, int f32, int T, int C, const int32_t* ids, int k,
                          const uint8_t* mask, float* out, int32_t* counts, float* frac, void* ws, size_t ws_bytes,
                          void* stream) {
-  RTE_REQUIRE(T >= 0 && C >= 1 && C <= kMaxPools && k >= 1 && ld >= 0, "pool_balance: need 1 <= pools <= %d and k >= 1",
-              kMaxPools);
+  RTE_REQUIRE(T >= 0 && C >= 1 && C <= kMaxPools && k >= 1 && k <= kMaxPools && ld >= 0,
+              "pool_balance: need 1 to %d pools and as many per row at most", kMaxPools);
   RTE_REQUIRE((int64_t)T * k < ((int64_t)1 << 31), "pool_balance: fewer than 2^31 (row, pool) pairs expected");
   RTE_REQUIRE((T == 0 || (logits && ids)) && out && counts && frac, "pool_balance: null argument");
   RTE_REQUIRE(ws_bytes >= rte_pool_balance_workspace_bytes(T, C) && (T == 0 || ws), "pool_balance: workspace too small");

@@ -1468,7 +1468,7 @@ def router_aux(probs, expected_depth, usage_ema, *, coverage_min: float, lambda_
 
 def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(balance, z, counts int32 [C]) of router logits [..., C] (float32 or bfloat16, C <= 1024) whose rows
-    were sent to the pools ids [..., k] (route_topk's; outside [0, C): none).
+    were sent to the pools ids [..., k] (route_topk's, k <= 1024; outside [0, C): none).
 
     balance = C sum_c f_c mean_t softmax(logits)_tc with f_c the share of the pairs that pool c got (1 when
     both are even), z = mean_t logsumexp(logits_t)^2.  mask (bool [...]) leaves rows out, padding for one,
@@ -1480,7 +1480,7 @@ def pool_balance(logits, ids, *, mask=None) -> tuple[torch.Tensor, torch.Tensor,
     lead = logits.shape[:-1]
     if logits.ndim < 1 or not 1 <= logits.shape[-1] <= 1024:
         raise ValueError(f"pool_balance: need [..., C] logits with 1 <= C <= 1024, got {tuple(logits.shape)}")
-    if ids.ndim < 1 or ids.shape[:-1] != lead or ids.shape[-1] < 1:
+    if ids.ndim < 1 or ids.shape[:-1] != lead or not 1 <= ids.shape[-1] <= 1024:
         raise ValueError(f"pool_balance: ids {tuple(ids.shape)} do not match logits {tuple(logits.shape)}")
     _whole_numbers("pool_balance", ids)
     if ids.numel() >= 1 << 31:
@@ -1711,6 +1711,8 @@ def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[to
         raise ValueError(f"lm_head_logprobs: hidden {tuple(hidden.shape)} and w {tuple(w.shape)} do not match")
     if tokens.shape != hidden.shape[:-1]:
         raise ValueError(f"lm_head_logprobs: tokens {tuple(tokens.shape)} do not match hidden {tuple(hidden.shape)}")
+    if w.shape[0] >= 1 << 30 or tokens.numel() >= 1 << 31:
+        raise ValueError(f"lm_head_logprobs: unsupported sizes {tuple(hidden.shape)}, {tuple(w.shape)}")
     t = _temperature("lm_head_logprobs", temperature)
     if fp32_active():
         return token_logprobs(_f32().linear(hidden, w), tokens, temperature=t)[:2]

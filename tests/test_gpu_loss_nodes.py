@@ -146,3 +146,11 @@ def test_errors_of_the_entry_points_reach_the_caller(H):
     ids = torch.zeros((T, 129), dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="rte_topk_distill_fwd failed"):
         _lib.ops().topk_distill(x, ids, ids.float(), 1.0, False, _lib.stream_ptr(x.device))
+
+
+def test_more_pools_per_row_than_there_can_be_are_refused(H):
+    x = torch.randn(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="pool_balance"):
+        H.pool_balance(x, torch.zeros((3, 1025), dtype=torch.int32, device="cuda"))
+    _, _, counts = H.pool_balance(x, torch.zeros((3, 1024), dtype=torch.int32, device="cuda"))
+    assert counts.tolist() == [3 * 1024] + [0] * 7

@@ -89,3 +89,9 @@ def test_pool_balance(lib):
     refused(lib, "rte_pool_balance_bwd", BUF, 64, 1, 4, 1025, None, BUF, None, None, BUF, None)
     refused(lib, "rte_pool_balance_bwd", BUF, 64, 1, 4, 64, None, None, None, None, BUF, None)
     assert lib.rte_pool_balance_bwd(None, 64, 1, 0, 64, None, None, None, None, None, None) == 0
+
+
+def test_pool_balance_lists_of_at_most_the_largest_pool_count(lib):
+    need = lib.rte_pool_balance_workspace_bytes(16, 64)
+    refused(lib, "rte_pool_balance_fwd", BUF, 64, 1, 16, 64, BUF, 1025, None, BUF, BUF, BUF, BUF, need, None)
+    refused(lib, "rte_pool_balance_fwd", BUF, 64, 1, 16, 64, BUF, (1 << 27) - 1, None, BUF, BUF, BUF, BUF, need, None)
