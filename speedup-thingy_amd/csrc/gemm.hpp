@@ -82,7 +82,10 @@ struct Epilogue {
   const int64_t* tokens = nullptr;   // [N]
   float4* row_part = nullptr;        // EPI_ROW_SUMS: [gemm_tile_row_blocks, N] {max, sum 2^u, sum 2^u u, -}, u in log2
   float* tok_logit = nullptr;        // EPI_ROW_SUMS: [N], written where the token is one of the columns
-  const float4* row_in = nullptr;    // EPI_DLOGITS: [N] {max, a, b, g / t}: d = 2^u (a + b u), u = x c2 - max
+  const float* row_stats = nullptr;  // EPI_DLOGITS: [N, 2] {max, log2 of the sum}, as EPI_ROW_SUMS's blocks joined
+  const float *row_entropy = nullptr, *g_lp = nullptr, *g_ent = nullptr;  // [N]; NULL gradients are 0
+  float inv_t = 0.0f;
+  int vocab = 0;                     // columns of the whole vocabulary
 };
 
 struct GemmArgs {

@@ -218,6 +218,23 @@ __device__ __forceinline__ void row_sums(const Epilogue& e, f32x16_v (&acc)[TM][
   }
 }
 
+// What the gradient of a row's logits needs of the row.  With l = log2 of e^{(x_v - m) / t}, m as rounded in the
+// sums, and S their total: p_v = 2^l / S and dx_v = 2^l (a + b l) + [v = token] g / t, where
+// b = -g_H ln 2 / (t S), a = -(g + g_H entropy) / (t S) - b log2 S.  terms() is {m, a, b, g / t}.
+struct RowIn {
+  float m, log_s, entropy, g, gh;
+  RowIn() = default;
+  __device__ __forceinline__ RowIn(const Epilogue& e, int n) {
+    m = e.row_stats[2 * (int64_t)n], log_s = e.row_stats[2 * (int64_t)n + 1], entropy = e.row_entropy[n];
+    g = e.g_lp ? e.g_lp[n] : 0.0f, gh = e.g_ent ? e.g_ent[n] : 0.0f;
+  }
+  __device__ __forceinline__ float4 terms(const Epilogue& e, int64_t tok) const {
+    const float gl = tok >= 0 && tok < e.vocab ? g * e.inv_t : 0.0f, ge = gh * e.inv_t;
+    const float inv_s = exp2_(-log_s), b = -ge * kLn2 * inv_s;
+    return make_float4(m, -(gl + ge * entropy) * inv_s - b * log_s, b, gl);
+  }
+};
+
 // Gradient of the logits of rows n .. n + 31 of h in the 64 vocabulary rows from m0 on, through a 4 KB patch so
 // that whole 128-byte lines leave.
 template <int J, int I0, int TM, int TN>
@@ -530,14 +547,14 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
     each_stage([&](auto s) { step(s, Young{}, std::true_type{}, kt + decltype(s)::value + ST); });
   // what the output needs of the rows of h is on its way during the last products
   int64_t tok[2] = {};
-  float4 row_in[2];
+  RowIn row_in[2];
   if constexpr (EPI == EPI_ROW_SUMS || EPI == EPI_DLOGITS) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       int n = n0 + wn * WTN + j * 32 + (lane & 31);
       n = n < p.N ? n : p.N - 1;
       tok[j] = p.epi.tokens[n];
-      if constexpr (EPI == EPI_DLOGITS) row_in[j] = p.epi.row_in[n];
+      if constexpr (EPI == EPI_DLOGITS) row_in[j] = RowIn(p.epi, n);
     }
   }
   each_stage([&](auto s) {
@@ -565,11 +582,12 @@ __global__ void __launch_bounds__(WM* WN * 64, (tile_wgs<BM, BN, WM, WN, BK, ST,
       else sums(std::false_type{});
     } else {
       unsigned char* patch = reinterpret_cast<unsigned char*>(pt);
-      dlogits64<0, 0>(e, acc, mw, mlim, nb, p.N, lane, patch, row_in[0], tok[0]);
-      dlogits64<1, 0>(e, acc, mw, mlim, nb + 32, p.N, lane, patch, row_in[1], tok[1]);
+      const float4 row[2] = {row_in[0].terms(e, tok[0]), row_in[1].terms(e, tok[1])};
+      dlogits64<0, 0>(e, acc, mw, mlim, nb, p.N, lane, patch, row[0], tok[0]);
+      dlogits64<1, 0>(e, acc, mw, mlim, nb + 32, p.N, lane, patch, row[1], tok[1]);
       if constexpr (TM == 4) {
-        dlogits64<0, 2>(e, acc, mw + 64, mlim, nb, p.N, lane, patch, row_in[0], tok[0]);
-        dlogits64<1, 2>(e, acc, mw + 64, mlim, nb + 32, p.N, lane, patch, row_in[1], tok[1]);
+        dlogits64<0, 2>(e, acc, mw + 64, mlim, nb, p.N, lane, patch, row[0], tok[0]);
+        dlogits64<1, 2>(e, acc, mw + 64, mlim, nb + 32, p.N, lane, patch, row[1], tok[1]);
       }
     }
     return;

@@ -6,7 +6,7 @@
 // sum of e u}: a 32nd of the fp32 logits; a second launch joins a row's blocks.  Sums and logarithms are in
 // units of log 2, relative to the rounded maximum itself.  Backward: the product again, whose epilogue writes the
 // logits' gradient in bf16 for the two products that follow (dh = dx w, dw = dx^T h).  Bound by the matrix units: 8192
-// tokens of d 1024, vocabulary 32768, 537 + 9 us forward, 558 + 5 + 446 + 18 + 433 backward; keeping the logits instead
+// tokens of d 1024, vocabulary 32768, 537 + 9 us forward, 558 + 446 + 18 + 433 backward; keeping the logits instead
 // of the second product would move 1 GB in bf16 both ways (400 us) and hold it from forward to backward.
 #include "../../include/rte_hip.h"
 #include "gemm_tile.hpp"
@@ -69,20 +69,6 @@ __global__ void __launch_bounds__(kRows* kSlices)
   stats[2 * t + 1] = log_s;
 }
 
-// What the backward's epilogue needs of a row.  With l = log2 of e^{(x_v - m) / t}, m as rounded in the sums, and S
-// their total: p_v = 2^l / S and dx_v = 2^l (a + b l) + [v = token] g / t, where
-// b = -g_H ln 2 / (t S), a = -(g + g_H entropy) / (t S) - b log2 S.
-__global__ void head_rows_kernel(int T, int V, const int64_t* __restrict__ tokens, const float* __restrict__ stats,
-                                 const float* __restrict__ entropy, const float* __restrict__ g_lp,
-                                 const float* __restrict__ g_ent, float inv_t, float4* __restrict__ rows) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= T) return;
-  const int64_t tok = tokens[t];
-  const float g = g_lp && tok >= 0 && tok < V ? g_lp[t] * inv_t : 0.0f, gh = g_ent ? g_ent[t] * inv_t : 0.0f;
-  const float log_s = stats[2 * t + 1], inv_s = exp2_(-log_s), b = -gh * kLn2 * inv_s;
-  rows[t] = make_float4(stats[2 * t], -(g + gh * entropy[t]) * inv_s - b * log_s, b, g);
-}
-
 // The product w h^T over n rows of w on the tile kernels.
 int tiles(const void* w, const void* h, int n, int T, int d, const Epilogue& e, int kind, hipStream_t s) {
   GemmArgs p;
@@ -140,10 +126,9 @@ struct Ranges {
 };
 
 struct BwdSpace {
-  size_t rows, grad, dh, pad, tail, gemm, total;
+  size_t grad, dh, pad, tail, gemm, total;
   BwdSpace(int T, int d, int V, const Ranges& r, bool h, bool w) {
-    rows = 0;
-    grad = up((size_t)T * sizeof(float4));
+    grad = 0;
     dh = grad + up((size_t)T * r.most() * sizeof(bf16));
     pad = dh + (h && !r.one() ? up((size_t)T * d * sizeof(float)) : 0);
     const bool ragged = r.rest8 != r.rest;
@@ -221,14 +206,10 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
   RTE_REQUIRE(ws && ws_bytes >= at.total, "lm_head_logprobs_bwd: workspace too small");
   auto s = static_cast<hipStream_t>(stream);
   char* base = static_cast<char*>(ws);
-  float4* rows = reinterpret_cast<float4*>(base + at.rows);
   void* grad = base + at.grad;
   void* gemm_ws = base + at.gemm;
   const size_t gemm_bytes = at.total - at.gemm;
   float* dh32 = reinterpret_cast<float*>(base + at.dh);
-  hipLaunchKernelGGL(head_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, s, T, V, tokens, stats, entropy, g_logprob,
-                     g_entropy, 1.0f / temperature, rows);
-  RTE_TRY(check_launch("lm_head_rows"));
   for (int lo = 0; lo < V;) {
     const bool last = lo == r.whole;  // the columns past the whole 64s
     int n = last ? r.rest8 : r.whole - lo < r.width ? r.whole - lo : r.width;
@@ -248,7 +229,12 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
     e.col0 = lo;
     e.cols = real;
     e.tokens = tokens;
-    e.row_in = rows;
+    e.row_stats = stats;
+    e.row_entropy = entropy;
+    e.g_lp = g_logprob;
+    e.g_ent = g_entropy;
+    e.inv_t = 1.0f / temperature;
+    e.vocab = V;
     RTE_TRY(tiles(wr, hidden, n, T, d, e, EPI_DLOGITS, s));
     if (dhidden)  // [T, n] [n, d]; in fp32 until the last of several ranges
       RTE_TRY(product(grad, n, 0, wr, d, 1, r.one() ? dhidden : dh32, !r.one(), T, d, n, lo > 0 ? 1.0f : 0.0f, gemm_ws,
