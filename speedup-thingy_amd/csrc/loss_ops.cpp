@@ -57,7 +57,8 @@ Tensor row_grad(const Tensor& g) { return g.defined() ? dense(g, at::kFloat) : g
 // A gradient that a graph of gradients (create_graph) may pass on, but not differentiate.
 Tensor once(Tensor dx, const char* op) {
   if (!at::GradMode::is_enabled() || !dx.defined()) return dx;
-  const auto stop = std::make_shared<torch::autograd::DelayedError>(std::string(op) + ": its gradient cannot be differentiated", 1);
+  const auto stop =
+      std::make_shared<torch::autograd::DelayedError>(std::string(op) + ": its gradient cannot be differentiated", 1);
   return stop->apply(variable_list{dx.requires_grad_()})[0];
 }
 

@@ -41,8 +41,8 @@ __device__ __forceinline__ bool soft_row(const Words* w, float (*v)[Row<X>::VE],
   return s != 0.0f;  // NaN rows take part
 }
 
-// Partials of a workgroup: [C] sums of p, [C] counts (both filled up to fours), sum of lse^2, rows.  Bound by reading the logits: a
-// wave keeps its columns' sums in registers over all its rows, 64 / LPR at a time, and the waves' sums
+// Partials of a workgroup: [C] sums of p, [C] counts (both filled up to fours), sum of lse^2, rows.  Bound by
+// reading the logits: a wave keeps its columns' sums in registers over all its rows, 64 / LPR at a time, and the waves' sums
 // meet in LDS at the end.  131071 x 256 fp32, top 16: 31 us, 4.6 TB/s (45 behind a backward pass, whose gradient is
 // still being written back); 8192 x 64, top 8: 4.8.
 template <class X, int LPR, int NV>
@@ -297,7 +297,10 @@ __global__ void __launch_bounds__(256)
 }
 
 // Rows of a forward workgroup: the fewest that keep the workgroups at one per CU.
-int64_t fwd_rows(int T) { return ((int64_t)T + kMaxBlocks - 1) / kMaxBlocks < 16 ? 16 : ((int64_t)T + kMaxBlocks - 1) / kMaxBlocks; }
+int64_t fwd_rows(int T) {
+  const int64_t rows = ((int64_t)T + kMaxBlocks - 1) / kMaxBlocks;
+  return rows < 16 ? 16 : rows;
+}
 int blocks(int T) { return (int)((T + fwd_rows(T) - 1) / fwd_rows(T)); }
 
 struct Call {

@@ -1720,7 +1720,8 @@ def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[to
         raise ValueError(f"lm_head_logprobs: the width must be a multiple of 8, got {w.shape[1]}")
     h = hidden.detach()
     hb = _aligned16(h.reshape(-1, h.shape[-1]).contiguous().to(BF16))
-    wb = _aligned16(cast_bf16(w).detach())
+    with _on_device(hidden.device):
+        wb = _aligned16(cast_bf16(w).detach())
     if _lib.load().rte_lm_head_logprobs_ok(hb.shape[0], hb.shape[1], wb.shape[0]):
         return _lib.ops().lm_head_logprobs(hidden, w, hb, wb, tokens, t, LMHeadLogprobsFn.GRAD,
                                            _lib.stream_ptr(hidden.device))
