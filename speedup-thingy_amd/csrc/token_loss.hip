@@ -506,21 +506,26 @@ __global__ void __launch_bounds__(256, TOP ? (E == 64 ? 4 : 6) : 8) rows_wave_ke
 
 // A range of a longer row in one pass of a workgroup: every lane keeps its own running maximum and sums over
 // batches of four vectors, the next of them on its way, and nothing is exchanged before the end.  Columns listed
-// (DIST) are left out by a bit mask in LDS.  For the alternatives (TOP) each lane leaves its maximum of every
-// batch in LDS; at the end the n-th largest of the 256 lanes' maxima is a threshold that n columns reach at
-// least, and only the few batches whose maximum reaches it are read again, four lanes each.
-// Bound by reading: 4096 x 131072 bf16 with 20 alternatives 195 us, 5.5 TB/s; 4099 x 32771 bf16 87 us behind a
-// backward pass, whose gradient is still being written back meanwhile, and 59 by itself.
+// (DIST) are left out by a bit mask in LDS.  For the alternatives (TOP) each lane leaves its maximum of every 32 of
+// its columns in LDS; at the end the n-th largest of the 256 lanes' maxima is a threshold that n columns reach at
+// least, and only the few 32s whose maximum reaches it are read again, a vector to a lane.
+// Bound by reading: 4096 x 131072 with 20 alternatives 205 us in bf16 and 370 in fp32, 5.2 and 5.8 TB/s; 4099 x 32771
+// bf16 87 us behind a backward pass, whose gradient is still being written back meanwhile, and 59 by itself.  Ranges of
+// 65536 and their join, with room for the longest range's maxima in every workgroup, took 219 us for the first,
+// 50 for 700 such rows (44 now) and 104 for 8000 x 9001 fp32 with 128 alternatives (88 now).
 constexpr int kBatch = 4;
-constexpr int kStreamCols = 65536;  // columns of a workgroup: 8 KB of bit mask, 16 batches of fp32
+constexpr int kStreamCols = 131072;  // columns of a workgroup: 16 KB of bit mask, or of maxima, one for 32 columns of a lane
+constexpr int kStreamMax = 32 * 256;  // columns to a row of those maxima
 constexpr int kItems = 512;
 
 template <class X, bool DIST, bool TOP>
 __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict__ logits, RowArgs a) {
   constexpr int VE = Row<X>::VE, COLS = kBatch * 256 * VE;
-  __shared__ uint32_t s_mask[DIST ? kStreamCols / 32 : 1];
+  constexpr int PER = 32 / (kBatch * VE);  // batches to a maximum
+  extern __shared__ uint32_t s_range[];  // as much as the range needs: what is left lets more workgroups in
+  uint32_t* s_mask = s_range;
+  float (*s_bmax)[256] = reinterpret_cast<float (*)[256]>(s_range);
   __shared__ Sums s_sums[4];
-  __shared__ float s_bmax[TOP ? kStreamCols / COLS : 1][TOP ? 256 : 1];
   __shared__ uint32_t s_key[TOP ? 256 : 1];
   __shared__ __align__(16) u64 s_cand[TOP ? kCandGroup : 1];
   __shared__ int s_items[TOP ? kItems : 1];
@@ -598,7 +603,8 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     r.s += s;
     if constexpr (TOP) {
       bm = s != s ? INFINITY : bm;  // a batch with NaN is always looked into
-      s_bmax[b / COLS][tid] = bm;
+      float& of = s_bmax[b / COLS / PER][tid];
+      of = b / COLS % PER ? fmaxf(of, bm) : bm;
       most = fmaxf(most, bm);
     }
   }
@@ -650,7 +656,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
       if (pos < kCandGroup) s_cand[pos] = raw_cand(x, c0 + off);
     };
     if (!(most < least)) {
-      for (int b = 0; b * COLS < len; ++b)
+      for (int b = 0; b * PER * COLS < len; ++b)
         if (!(s_bmax[b][tid] < least)) {
           const int pos = atomicAdd(&s_ctl[0], 1);
           if (pos < kItems) s_items[pos] = b * 256 + tid;
@@ -659,8 +665,9 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
     __syncthreads();
     const int items = s_ctl[0];
     if (items <= kItems) {
-      for (int q = tid; q < items * kBatch; q += 256) {
-        const int it = s_items[q / kBatch], off = (it >> 8) * COLS + ((q % kBatch) * 256 + (it & 255)) * VE;
+      for (int q = tid; q < items * PER * kBatch; q += 256) {
+        const int it = s_items[q / (PER * kBatch)], v0 = q % (PER * kBatch);
+        const int off = ((it >> 8) * PER + v0 / kBatch) * COLS + ((v0 % kBatch) * 256 + (it & 255)) * VE;
         const Words v = load_words(at, off, len);
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
@@ -753,7 +760,7 @@ __global__ void __launch_bounds__(256, 6) rows_stream_kernel(const X* __restrict
 }
 
 // Joins a row's ranges: sums rescaled to the common maximum, the alternatives merged by rank (a key's rank is
-// the number of larger keys in every range's sorted list).  4096 rows of two ranges, 20 alternatives: 11 us.
+// the number of larger keys in every range's sorted list).  4096 rows of two ranges, 20 alternatives: 11 us, most of it the rows' dependent reads.
 constexpr int kJoinKeys = 2048;
 template <class X, bool DIST, bool TOP>
 __global__ void __launch_bounds__(TOP ? 256 : 64) rows_join_kernel(const X* __restrict__ logits, RowArgs a) {
@@ -930,7 +937,8 @@ int launch_rows(const void* logits, RowArgs a, void* ws, hipStream_t s) {
   RTE_REQUIRE(grid < ((int64_t)1 << 31), "token_loss: too many rows");
   a.part_stats = static_cast<float4*>(ws);
   a.part_keys = reinterpret_cast<u64*>(a.part_stats + grid);
-  hipLaunchKernelGGL((rows_stream_kernel<X, DIST, TOP>), dim3((unsigned)grid), dim3(256), 0, s, x, a);
+  const int words = DIST ? (a.part + 31) / 32 : TOP ? (a.part + kStreamMax - 1) / kStreamMax * 256 : 0;
+  hipLaunchKernelGGL((rows_stream_kernel<X, DIST, TOP>), dim3((unsigned)grid), dim3(256), words * sizeof(uint32_t), s, x, a);
   RTE_TRY(check_launch("token_loss_stream"));
   if (a.nparts == 1) return 0;
   hipLaunchKernelGGL((rows_join_kernel<X, DIST, TOP>), dim3(a.T), dim3(TOP ? 256 : 64), 0, s, x, a);

@@ -712,3 +712,45 @@ def test_distill_nothing_outside_the_list(H, V, repeat):
     many = lambda v: v.repeat(repeat, 1)
     check_distill(H, many(x), many(ids), many(tl), 1.0, False, g)
     check_distill(H, many(x).bfloat16(), many(ids), many(tl), 2.0, False, g)
+
+
+# ----------------------------------------------------------------------------- enough rows for one range each
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,V,n_top", [(513, 131072, 5), (520, 131071, 128), (513, 140001, 33), (700, 8193, 100)])
+def test_longest_single_range(H, T, V, n_top, dtype):
+    """One workgroup's whole room for a row, all but a column of it, and a second range; ties in the last columns, in one
+    lane's and everywhere."""
+    g = gen(T, V, dtype, 22)
+    x = torch.randn(T, V, device=DEV, generator=g).to(DT[dtype])
+    x[1, -3:] = 9.0
+    x[2, 64:V:8192] = 7.0
+    x[3, ::2] = 6.0
+    x[4] = 1.0
+    x[5, : V - 2] = -math.inf
+    tok = torch.randint(0, V, (T,), device=DEV, generator=g)
+    tok[:6] = V - 1
+    check_logprobs(H, x, tok, n_top, 1.0, g)
+
+
+@pytest.mark.parametrize("V", [131072, 140001])
+def test_distill_longest_single_range(H, V):
+    """520 rows take one range each (two past 131072 columns), eight of them many short ones: the same results, within
+    the tolerances of both."""
+    g = gen(V, 23)
+    x = torch.randn(8, V, device=DEV, generator=g) * 2
+    ids, tl = teacher(x, 100, 1.0, True, g)
+    ids[0, 0], ids[1, 5] = V - 1, ids[1, 9]
+    check_distill(H, x, ids, tl, 1.0, True, g)
+    leaf = x.detach().requires_grad_()
+    few = H.topk_distill(leaf, ids, tl, tail=True)
+    (d_few,) = torch.autograd.grad(few.sum(), leaf)
+    many = x.repeat(65, 1).requires_grad_()
+    loss = H.topk_distill(many, ids.repeat(65, 1), tl.repeat(65, 1), tail=True)
+    (dx,) = torch.autograd.grad(loss.sum(), many)
+    c = ulps(V, 2 * 12.0)
+    near(loss.view(65, 8), few.expand(65, 8), 2 * (2 * c + 2.0 ** -22 * few.detach().double().abs()), "loss")
+    q = torch.softmax(x.double(), 1)
+    p = torch.zeros_like(q).scatter_(1, ids, tl.double().exp())
+    tol = 2 * (8 * c * (2 * q + p) + 2.0 ** -21 * q) + 1e-37
+    near(dx.view(65, 8, V), d_few.expand(65, 8, V), tol.expand(65, 8, V), "gradient")
