@@ -5,8 +5,9 @@
 // for 12 us of kernels (autograd's thread waits for the interpreter), with these 62.  Log probabilities from hidden
 // states: 172 and 101 us; without gradients, 17 and 8 us for log probabilities from logits.
 //
-// Arguments are checked by the Python wrappers (rte_amd/kernels/hip_ops.py) before they come here.  `stream` is the
-// current stream on the operands' device: a node's backward runs on the stream of its forward, so it is kept for that.
+// The Python wrappers (rte_amd/kernels/hip_ops.py) check arguments with the framework's errors; here only what a kernel
+// could not survive is checked again.  `stream` is the current stream on the operands' device: a node's backward runs
+// on the stream of its forward, so it is kept for that.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -27,6 +28,18 @@ void ok(int rc, const char* entry) { TORCH_CHECK(rc == 0, entry, " failed (code 
 
 Tensor dense(const Tensor& t, at::ScalarType dtype) {
   return t.scalar_type() == dtype && t.is_contiguous() ? t : t.contiguous().to(dtype);
+}
+
+// Rows x [..., V] on a device, in a type of the kernels.
+void check_rows(const char* op, const Tensor& x) {
+  TORCH_CHECK(x.is_cuda(), op, ": expects ROCm device tensors");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && (x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16), op,
+              ": float32 or bfloat16 rows expected");
+}
+// An operand of n values for every row of x.
+void check_beside(const char* op, const Tensor& x, const Tensor& t, int64_t n) {
+  TORCH_CHECK(t.device() == x.device() && n >= 1 && t.numel() == x.numel() / x.size(-1) * n, op,
+              ": an operand does not match the rows");
 }
 
 // Ids in 32 bits; wider ones that do not fit stay out of every range.
@@ -72,6 +85,9 @@ struct Logprobs {
 };
 
 Logprobs logprobs(const Tensor& logits, const Tensor& tokens, int64_t n_top, double temperature, bool need, int64_t stream) {
+  check_rows("token_logprobs", logits);
+  check_beside("token_logprobs", logits, tokens, 1);
+  TORCH_CHECK(n_top >= 0 && n_top <= logits.size(-1), "token_logprobs: n_top must be in [0, V]");
   c10::DeviceGuard guard(logits.device());
   Logprobs r;
   std::tie(r.rows, r.ld) = rows_of(logits);
@@ -144,6 +160,10 @@ struct Distill {
 
 Distill distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, double temperature, bool tail, bool need,
                 int64_t stream) {
+  check_rows("topk_distill", logits);
+  TORCH_CHECK(ids.dim() >= 1, "topk_distill: lists expected");
+  check_beside("topk_distill", logits, ids, ids.size(-1));
+  check_beside("topk_distill", logits, teacher, ids.size(-1));
   c10::DeviceGuard guard(logits.device());
   Distill r;
   std::tie(r.rows, r.ld) = rows_of(logits);
@@ -204,6 +224,13 @@ Tensor topk_distill(const Tensor& logits, const Tensor& ids, const Tensor& teach
 struct PoolBalance : Function<PoolBalance> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, const OptTensor& mask,
                                int64_t stream) {
+    check_rows("pool_balance", logits);
+    TORCH_CHECK(ids.dim() >= 1, "pool_balance: lists expected");
+    check_beside("pool_balance", logits, ids, ids.size(-1));
+    if (mask) {
+      check_beside("pool_balance", logits, *mask, 1);
+      TORCH_CHECK(mask->scalar_type() == at::kBool, "pool_balance: mask must be bool");
+    }
     c10::DeviceGuard guard(logits.device());
     const auto [rows, ld] = rows_of(logits);
     const int64_t C = logits.size(-1), k = ids.size(-1), T = ids.numel() / k;
@@ -254,6 +281,14 @@ struct HeadLogprobs : Function<HeadLogprobs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& hb,
                                const Tensor& wb, const Tensor& tokens, double temperature, int64_t grad_bytes,
                                int64_t stream) {
+    for (const Tensor* t : {&hb, &wb}) {
+      check_rows("lm_head_logprobs", *t);
+      TORCH_CHECK(t->dim() == 2 && t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->size(1) == hb.size(1) &&
+                      t->device() == hb.device(),
+                  "lm_head_logprobs: dense bfloat16 matrices of one width expected");
+    }
+    check_beside("lm_head_logprobs", hb, tokens, 1);
+    TORCH_CHECK(hidden.numel() == hb.numel() && w.sizes() == wb.sizes(), "lm_head_logprobs: the copies do not match");
     c10::DeviceGuard guard(hb.device());
     const Tensor tk = dense(tokens, at::kLong);
     const int64_t T = hb.size(0), d = hb.size(1), V = wb.size(0);

@@ -154,3 +154,21 @@ def test_more_pools_per_row_than_there_can_be_are_refused(H):
         H.pool_balance(x, torch.zeros((3, 1025), dtype=torch.int32, device="cuda"))
     _, _, counts = H.pool_balance(x, torch.zeros((3, 1024), dtype=torch.int32, device="cuda"))
     assert counts.tolist() == [3 * 1024] + [0] * 7
+
+
+def test_operands_that_do_not_match_are_refused_by_the_nodes(H):
+    from rte_amd import _lib
+
+    ops = _lib.ops()
+    x, tok, ids, tl, h, w = operands()
+    s = _lib.stream_ptr(x.device)
+    bad = [lambda: ops.token_logprobs(x, tok[1:], 0, 1.0, s), lambda: ops.token_logprobs(x, tok.cpu(), 0, 1.0, s),
+           lambda: ops.token_logprobs(x.half(), tok, 0, 1.0, s), lambda: ops.token_logprobs(x, tok, -1, 1.0, s),
+           lambda: ops.topk_distill(x, ids[1:], tl, 1.0, False, s), lambda: ops.topk_distill(x, ids, tl[:, 1:], 1.0, False, s),
+           lambda: ops.pool_balance(x, ids[1:], None, s), lambda: ops.pool_balance(x, ids, tok, s),
+           lambda: ops.lm_head_logprobs(h, w, h, w[:, :64], tok, 1.0, 1 << 20, s),
+           lambda: ops.lm_head_logprobs(h, w, h.float(), w, tok, 1.0, 1 << 20, s),
+           lambda: ops.lm_head_logprobs(h, w, h, w, tok[1:], 1.0, 1 << 20, s)]
+    for call in bad:
+        with pytest.raises(RuntimeError):
+            call()

@@ -95,3 +95,20 @@ def test_pool_balance_lists_of_at_most_the_largest_pool_count(lib):
     need = lib.rte_pool_balance_workspace_bytes(16, 64)
     refused(lib, "rte_pool_balance_fwd", BUF, 64, 1, 16, 64, BUF, 1025, None, BUF, BUF, BUF, BUF, need, None)
     refused(lib, "rte_pool_balance_fwd", BUF, 64, 1, 16, 64, BUF, (1 << 27) - 1, None, BUF, BUF, BUF, BUF, need, None)
+
+
+def test_the_nodes_refuse_what_a_kernel_could_not_survive():
+    """The registered operators, called past their Python wrappers: operands off the device, for one."""
+    import torch
+
+    from rte_amd import _lib
+
+    ops = _lib.ops()
+    x, tok, ids = torch.zeros(4, 8), torch.zeros(4, dtype=torch.long), torch.zeros(4, 2, dtype=torch.int32)
+    for needs in (False, True):
+        leaf = x.clone().requires_grad_(needs)
+        for call in (lambda: ops.token_logprobs(leaf, tok, 0, 1.0, 0), lambda: ops.topk_distill(leaf, ids, ids.float(), 1.0, False, 0),
+                     lambda: ops.pool_balance(leaf, ids, None, 0),
+                     lambda: ops.lm_head_logprobs(leaf, leaf, leaf.detach().bfloat16(), leaf.detach().bfloat16(), tok, 1.0, 1 << 20, 0)):
+            with pytest.raises(RuntimeError, match="device tensors"):
+                call()
