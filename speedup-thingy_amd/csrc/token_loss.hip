@@ -907,8 +907,9 @@ __global__ void __launch_bounds__(256)
 }
 
 // Rows that one wave holds in 32 registers or fewer, where there are four waves of them for every CU; a row of its
-// own workgroup otherwise.  (65536 rows, 20 alternatives, wave / workgroup in us: bf16 x 4096 208 / 290, x 3000
-// 177 / 271, fp32 x 4096, 64 registers, 319 / 310; one bf16 row of 3000 8.8 / 6.3.)
+// own workgroup otherwise.  (20 alternatives, wave / workgroup in us: 65536 rows of bf16 x 4096 245 / 289, x 3000
+// 194 / 261, of fp32 x 2048 145 / 228; 8192 rows 34 / 37, -, 26 / 32; 1100 rows 12 / 11, -, 11 / 11; fp32 x 4096, in 64
+// registers, 65536 rows 319 / 310; one bf16 row of 3000 8.8 / 6.3.)
 bool by_wave(int T, int V, bool f32) { return T >= 1024 && V <= (f32 ? 2048 : 4096); }
 
 // Ranges of a row: a workgroup takes up to kStreamCols columns, and rows too few to give every CU two workgroups
