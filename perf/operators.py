@@ -16,7 +16,6 @@ the framework.  `exact` restates the definitions in 64 bits.
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -184,7 +183,6 @@ def prepare(case, seed):
 
 # ----------------------------------------------------------------------------- one pass
 
-@functools.cache
 def _ops():
     pkg = str(Path(__file__).resolve().parent.parent / "speedup-thingy_amd")
     if pkg not in sys.path:
