@@ -670,8 +670,9 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
  * A row without entries (tail 0: or without one above -inf) has loss 0 and no gradient; an id past the
  * vocabulary makes the loss NaN and the gradient 0.  K <= 128.
  * Kept for the backward (stats NULL: nothing is): stats f32 [T, 2], cols int32 [T, K] = the columns that count
- * (-1: none), coef f32 [T, K] = q - p there.
- * bwd: dlogits [T, V] dense in the logits' type, for g f32 [T]. */
+ * (-1: none), coef f32 [T, K] = n q - p there, n = sum p_j + r (1 but for lists that sum to more).
+ * bwd: dlogits [T, V] dense in the logits' type, for g f32 [T]: with n as above temperature g (n q - p) on the
+ * list, temperature g (n q - r q / q(not listed)) off it. */
 size_t rte_topk_distill_workspace_bytes(int T, int V, int K);
 int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, const int32_t* ids,
                          const float* teacher, int K, float temperature, int tail, float* loss, float* stats,

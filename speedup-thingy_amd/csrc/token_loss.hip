@@ -11,7 +11,9 @@
 //
 //   tail 0: p = softmax_j(t_j / t)           L = t^2 sum_j p_j (log p_j - log q_{c_j})
 //   tail 1: p_j = e^{t_j}, r = 1 - sum p_j   L = t^2 (sum_j p_j (log p_j - log q_{c_j}) + r (log r - log q(R)))
-//   dx_v  = g t (q_v - p_j) where v = c_j, else g t (q_v - r q_v / q(R)) (tail 0: r = 0)
+//   dx_v  = g t (n q_v - p_j) where v = c_j, else g t (n q_v - r q_v / q(R)) (tail 0: r = 0)
+//
+// with r never below 0 and n = sum p_j + r: 1 but for lists whose exponentials (tail 1) sum to more.
 #include "../../include/rte_hip.h"
 #include "row_words.hpp"
 
@@ -199,6 +201,7 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
       p[i] *= tinv;
     }
   }
+  const double mass = a.tail ? tsum + r : 1.0;
   const bool empty = total == 0.0;
   double l = 0.0;
 #pragma unroll
@@ -214,15 +217,15 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   if (lane == 0) {
     const bool out = none || rest.s == 0.0f;  // no column outside the list above -inf
     a.stats[2 * t] = out ? 0.0f : rest.m;
-    // (q(R) - r) / (the rest's sum relative to its own maximum)
-    a.stats[2 * t + 1] = out ? 0.0f : (float)((rsum * inv - r) / rest.s);
+    // (mass q(R) - r) / (the rest's sum relative to its own maximum)
+    a.stats[2 * t + 1] = out ? 0.0f : (float)((rsum * inv * mass - r) / rest.s);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int j = lane + 64 * i;
     if (j >= a.K) continue;
     a.cols[t * a.K + j] = none ? -1 : col[i];
-    a.coef[t * a.K + j] = none ? 0.0f : (float)(e[i] * inv - p[i]);
+    a.coef[t * a.K + j] = none ? 0.0f : (float)(e[i] * inv * mass - p[i]);
   }
 }
 

@@ -1,0 +1,127 @@
+"""topk_distill(tail=True): what a list leaves of 1, in loss and gradient, against 64-bit autograd of the definition
+
+    loss = t^2 (sum_j p_j (log p_j - log q_j) + r (log r - log q(R))),  p_j = e^{t_j},  r = max(1 - sum p_j, 0)
+
+R the columns not listed.
+
+Tolerances, from the arithmetic: the sum of the exponentials off the list is right to C = 2^-24 (V / 256 + 16 + 4 max |u|) of
+itself (see `ulps`), everything of the list is computed in 64 bits, and each result is rounded once."""
+
+from __future__ import annotations
+
+import math
+import zlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F64 = torch.float64
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module")
+def H():
+    from rte_amd.kernels import hip_ops
+
+    return hip_ops
+
+
+def gen(*seed):
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(seed).encode()))
+
+
+def ulps(V, umax):
+    return 2.0 ** -24 * (V / 256 + 16 + 4 * umax)
+
+
+def loss64(z, ids, tl):
+    """The definition for z = logits / t (double), ids without repeats, every row with an entry; its loss / t^2, and the sum of
+    its terms' sizes."""
+    lq = torch.log_softmax(z, 1)
+    here = ids >= 0
+    at = ids.clamp_min(0).long()
+    p = torch.where(here, tl.to(F64).exp(), 0.0)
+    terms = torch.where(p > 0, p * (tl.to(F64) - lq.gather(1, at)), 0.0)
+    on = torch.zeros_like(z).scatter_add_(1, at, here.to(F64)) > 0
+    off = lq.masked_fill(on, -math.inf)
+    reach = (off > -math.inf).any(1)
+    r = (1.0 - p.sum(1)).clamp_min(0.0)
+    # the logarithm of nothing is left out of the graph where it is not read
+    lqr = torch.where(reach, torch.logsumexp(torch.where(reach[:, None], off, 0.0), 1), -math.inf)
+    rest = torch.where(r > 0, r * (torch.where(r > 0, r, 1.0).log() - torch.where(r > 0, lqr, 0.0)), 0.0)
+    sizes = terms.abs().sum(1) + torch.where(r > 0, rest.abs(), 0.0)
+    return terms.sum(1) + rest, sizes
+
+
+def check(H, x, ids, tl, t, g):
+    T, V = x.shape
+    up = torch.rand(T, device=DEV, generator=g) + 0.5
+    leaf = x.detach().requires_grad_()
+    loss = H.topk_distill(leaf, ids, tl, temperature=t, tail=True)
+    (dx,) = torch.autograd.grad(loss, leaf, up)
+    z = (x.to(F64) / t).requires_grad_()
+    want, sizes = loss64(z, ids, tl)
+    want, sizes = want * t * t, sizes.detach() * t * t
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(loss), fin), "finite at other rows"
+    assert torch.equal(loss.detach()[~fin].to(F64), want.detach()[~fin]), "infinities"
+    u = z.detach().amax(1, keepdim=True) - z.detach()
+    c = ulps(V, float(u[u < 200].max()))
+    err = (loss.detach().to(F64) - want.detach()).abs() - (2 * c + HALF[torch.float32] * 2) * (sizes + t * t)
+    assert float(err[fin].max()) <= 0, f"loss off by {float(err[fin].max()):.3g} over the tolerance"
+    if not bool(fin.all()):
+        return loss, dx
+    (dz,) = torch.autograd.grad(want, z, up.to(F64))
+    d = dz / t
+    # the terms of a column: mass q, p and the rest's share, each right to c and a few roundings of fp32
+    q = torch.softmax(z.detach(), 1)
+    p = torch.zeros_like(q).scatter_add_(1, ids.clamp_min(0).long(), torch.where(ids >= 0, tl.to(F64).exp(), 0.0))
+    mass = p.sum(1, keepdim=True).clamp_min(1.0)
+    off = z.detach().masked_fill(p > 0, -math.inf)
+    some = (off > -math.inf).any(1, keepdim=True)
+    rest = torch.where(some, (1 - p.sum(1, keepdim=True)).clamp_min(0.0) * torch.softmax(torch.where(some, off, 0.0), 1), 0.0)
+    scale = (mass * q + p + rest) * up.to(F64)[:, None] * t
+    tol = (8 * c + 2.0 ** -21) * scale + HALF[x.dtype] * d.abs() + 1e-37
+    err = (dx.to(F64) - d).abs() - tol
+    assert float(err.max()) <= 0, f"gradient off by {float(err.max()):.3g} over the tolerance"
+    return loss, dx
+
+
+ROWS = [(5, 40, 5), (1030, 40, 5), (6, 2048, 16), (1027, 2047, 64), (1026, 4000, 7), (7, 9001, 33), (3, 70001, 128)]
+
+
+def lists(T, V, K, g):
+    return torch.stack([torch.randperm(V, device=DEV, generator=g)[:K] for _ in range(T)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("total", [1.0001, 1.02, 1.5, 4.0])
+@pytest.mark.parametrize("T,V,K", ROWS)
+def test_lists_that_sum_to_more_than_one(H, T, V, K, total, dtype):
+    """Nothing is left for the rest, and the student's probabilities weigh as much as the whole list: a row's gradient
+    sums to 0."""
+    g = gen(T, V, K, total, 1)
+    t = 2.0 if K % 2 else 0.7
+    x = (torch.randn(T, V, device=DEV, generator=g) * 2).to(dtype)
+    ids = lists(T, V, K, g)
+    tl = torch.log_softmax(torch.randn(T, K, device=DEV, generator=g), 1) + math.log(total)
+    check(H, x, ids, tl, t, g)
+
+
+@pytest.mark.parametrize("T,V", [(9, 2), (1100, 2), (9, 300), (1100, 300), (9, 9001)])
+def test_alternatives_kept_in_bf16(H, T, V):
+    """token_logprobs' alternatives rounded to 16 bits: two near-even ones sum to 1.0017 or 0.998."""
+    g = gen(T, V, 2)
+    y = torch.full((T, V), -30.0, device=DEV)
+    y[:, :2] = torch.randn(T, 2, device=DEV, generator=g) * 0.3
+    _, _, tl, ids = H.token_logprobs(y, torch.zeros(T, dtype=torch.long, device=DEV), n_top=2)
+    kept = tl.bfloat16()
+    sums = kept.float().exp().sum(1)
+    assert bool((sums > 1.0005).any()) and bool((sums < 0.9995).any())
+    x = torch.randn(T, V, device=DEV, generator=g)
+    if V == 2:  # what is left is then out of reach: only the rows without it have a finite loss
+        kept, ids, x = kept[sums > 1.0005], ids[sums > 1.0005], x[sums > 1.0005]
+    check(H, x, ids, kept, 1.0, g)
