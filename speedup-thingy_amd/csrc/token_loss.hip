@@ -190,7 +190,8 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   if (rest.m == -INFINITY && rest.s != 0.0f) rsum = __builtin_nan("");
   const double total = wave_sum(e[0] + e[1]) + rsum, tsum = wave_sum(p[0] + p[1]);
   const double r = a.tail ? (tsum > 1.0 ? 0.0 : 1.0 - tsum) : 0.0;
-  const double logs = log(lane == 0 ? total : lane == 1 ? tsum : lane == 2 ? r : rsum);
+  // the rest's own sum: times its scale it may be below the least number, however finite its logarithm
+  const double logs = log(lane == 0 ? total : lane == 1 ? tsum : lane == 2 ? r : (double)rest.s);
   const double inverses = 1.0 / (lane == 0 ? total : tsum);
   const double log_s = of_lane(logs, 0), inv = of_lane(inverses, 0);
   if (!a.tail) {
@@ -210,7 +211,7 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
     if (col[i] >= 0 && p[i] != 0.0) l += p[i] * (lp[i] - lq);
   }
   l = wave_sum(l);
-  if (r > 0.0) l += r * (of_lane(logs, 2) - (empty ? -INFINITY : of_lane(logs, 3) - log_s));
+  if (r > 0.0) l += r * (of_lane(logs, 2) - (rest.s == 0.0f ? -INFINITY : to_rest + of_lane(logs, 3) - log_s));
   if (lane == 0) a.loss[t] = foreign ? __builtin_nanf("") : some ? (float)(l * a.t2) : 0.0f;
   if (!a.stats) return;
   const bool none = foreign || !some || empty;

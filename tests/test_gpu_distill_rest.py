@@ -49,8 +49,10 @@ def loss64(z, ids, tl):
     off = lq.masked_fill(on, -math.inf)
     reach = (off > -math.inf).any(1)
     r = (1.0 - p.sum(1)).clamp_min(0.0)
-    # the logarithm of nothing is left out of the graph where it is not read
-    lqr = torch.where(reach, torch.logsumexp(torch.where(reach[:, None], off, 0.0), 1), -math.inf)
+    # relative to the largest, which a logarithm of -1e38 and the count of columns would swallow; the logarithm of nothing is
+    # left out of the graph where it is not read
+    top = torch.where(reach, off.detach().amax(1), 0.0)
+    lqr = torch.where(reach, top + torch.where(reach[:, None], off - top[:, None], 0.0).exp().sum(1).log(), -math.inf)
     rest = torch.where(r > 0, r * (torch.where(r > 0, r, 1.0).log() - torch.where(r > 0, lqr, 0.0)), 0.0)
     sizes = terms.abs().sum(1) + torch.where(r > 0, rest.abs(), 0.0)
     return terms.sum(1) + rest, sizes
@@ -125,3 +127,20 @@ def test_alternatives_kept_in_bf16(H, T, V):
     if V == 2:  # what is left is then out of reach: only the rows without it have a finite loss
         kept, ids, x = kept[sums > 1.0005], ids[sums > 1.0005], x[sums > 1.0005]
     check(H, x, ids, kept, 1.0, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", [-800.0, -1e4, -1e9, "lowest"])
+@pytest.mark.parametrize("T,V,K", ROWS)
+def test_rest_far_below_the_list(H, T, V, K, low, dtype):
+    """A student whose unlisted columns are masked by a large negative value: they can still be reached, and the loss of
+    the mass that the teacher leaves to them is large and finite."""
+    g = gen(T, V, K, low, 3)
+    low = float(torch.finfo(dtype).min) if low == "lowest" else low
+    ids = lists(T, V, K, g)
+    x = torch.full((T, V), low, device=DEV, dtype=dtype)
+    x.scatter_(1, ids, torch.randn(T, K, device=DEV, generator=g).to(dtype))
+    tl = torch.log_softmax(torch.randn(T, K, device=DEV, generator=g), 1) + math.log(0.75)
+    t = 1.0 if K % 2 else 0.5  # a quarter of t |low| fits the loss's type
+    loss, _ = check(H, x, ids, tl, t, g)
+    assert bool(torch.isfinite(loss).all()) and float(loss.detach().min()) > 0.2 * t * -low
