@@ -13,7 +13,8 @@
 //   tail 1: p_j = e^{t_j}, r = 1 - sum p_j   L = t^2 (sum_j p_j (log p_j - log q_{c_j}) + r (log r - log q(R)))
 //   dx_v  = g t (n q_v - p_j) where v = c_j, else g t (n q_v - r q_v / q(R)) (tail 0: r = 0)
 //
-// with r never below 0 and n = sum p_j + r: 1 but for lists whose exponentials (tail 1) sum to more.
+// with r never below 0, taken as 0 where it is rounding and q(R) is 0, and n = sum p_j + r: 1 but for lists whose
+// exponentials (tail 1) sum to more.
 #include "../../include/rte_hip.h"
 #include "row_words.hpp"
 
@@ -189,7 +190,11 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   double rsum = rest.s == 0.0f ? 0.0 : rest.s * scale;  // a NaN sum stays
   if (rest.m == -INFINITY && rest.s != 0.0f) rsum = __builtin_nan("");
   const double total = wave_sum(e[0] + e[1]) + rsum, tsum = wave_sum(p[0] + p[1]);
-  const double r = a.tail ? (tsum > 1.0 ? 0.0 : 1.0 - tsum) : 0.0;
+  double r = a.tail ? (tsum > 1.0 ? 0.0 : 1.0 - tsum) : 0.0;
+  // What roundings leave of 1 is no mass outside the list, which would make the loss infinite where the student can have
+  // none there.  fp32 log probabilities of a row with K possible columns leave at most 2^-24 (K + 2 + 7 log K): K + 2 from
+  // the exponentials and their sum, the rest from exponents, logarithm and results, each weighted by p; log K < 5.
+  if (rest.s == 0.0f && r <= (a.K + 32) * 0x1p-23) r = 0.0;
   // the rest's own sum: times its scale it may be below the least number, however finite its logarithm
   const double logs = log(lane == 0 ? total : lane == 1 ? tsum : lane == 2 ? r : (double)rest.s);
   const double inverses = 1.0 / (lane == 0 ? total : tsum);

@@ -2,7 +2,8 @@
 
     loss = t^2 (sum_j p_j (log p_j - log q_j) + r (log r - log q(R))),  p_j = e^{t_j},  r = max(1 - sum p_j, 0)
 
-R the columns not listed.
+R the columns not listed; where R cannot be reached, an r within the rounding of the list's log probabilities, 2^-23 (K + 32),
+is 0.
 
 Tolerances, from the arithmetic: the sum of the exponentials off the list is right to C = 2^-24 (V / 256 + 16 + 4 max |u|) of
 itself (see `ulps`), everything of the list is computed in 64 bits, and each result is rounded once."""
@@ -37,6 +38,10 @@ def ulps(V, umax):
     return 2.0 ** -24 * (V / 256 + 16 + 4 * umax)
 
 
+def bound(K):
+    return 2.0 ** -23 * (K + 32)
+
+
 def loss64(z, ids, tl):
     """The definition for z = logits / t (double), ids without repeats, every row with an entry; its loss / t^2, and the sum of
     its terms' sizes."""
@@ -49,6 +54,7 @@ def loss64(z, ids, tl):
     off = lq.masked_fill(on, -math.inf)
     reach = (off > -math.inf).any(1)
     r = (1.0 - p.sum(1)).clamp_min(0.0)
+    r = torch.where(~reach & (r <= bound(ids.shape[1])), 0.0, r)
     # relative to the largest, which a logarithm of -1e38 and the count of columns would swallow; the logarithm of nothing is
     # left out of the graph where it is not read
     top = torch.where(reach, off.detach().amax(1), 0.0)
@@ -144,3 +150,58 @@ def test_rest_far_below_the_list(H, T, V, K, low, dtype):
     t = 1.0 if K % 2 else 0.5  # a quarter of t |low| fits the loss's type
     loss, _ = check(H, x, ids, tl, t, g)
     assert bool(torch.isfinite(loss).all()) and float(loss.detach().min()) > 0.2 * t * -low
+
+
+ALL_LISTED = [(2000, 1), (2000, 2), (50, 5), (2000, 5), (2000, 17), (40, 64), (1500, 64), (1200, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [0.7, 1.0, 2.0])
+@pytest.mark.parametrize("T,V", ALL_LISTED)
+def test_every_column_listed(H, T, V, t, dtype):
+    """token_logprobs' own alternatives, all of them: what the roundings of their log probabilities leave of 1 is no mass
+    outside the list."""
+    g = gen(T, V, t, 4)
+    y = (torch.randn(T, V, device=DEV, generator=g) * 2).to(dtype)
+    _, _, tl, ids = H.token_logprobs(y, torch.zeros(T, dtype=torch.long, device=DEV), n_top=V, temperature=t)
+    loss, dx = check(H, y, ids, tl, t, g)
+    # each log probability is off by less than the bound on what they leave of 1, and the p_j sum to 1
+    assert float(loss.detach().abs().max()) <= bound(V) * t * t
+    x = (torch.randn(T, V, device=DEV, generator=g) * 2).to(dtype)
+    loss, _ = check(H, x, ids, tl, t, g)
+    assert bool(torch.isfinite(loss).all())
+
+
+@pytest.mark.parametrize("T,V,n", [(60, 300, 3), (1100, 300, 20), (1100, 2048, 64), (60, 9001, 100), (40, 70001, 17)])
+def test_all_but_the_listed_columns_banned(H, T, V, n):
+    """A teacher and a student that ban the same columns; the list has room for the rest and a few places more."""
+    g = gen(T, V, n, 5)
+    allowed = torch.randperm(V, device=DEV, generator=g)[:n]
+    banned = torch.ones(V, dtype=torch.bool, device=DEV)
+    banned[allowed] = False
+    y = torch.randn(T, V, device=DEV, generator=g).masked_fill(banned, -math.inf)
+    x = torch.randn(T, V, device=DEV, generator=g).masked_fill(banned, -math.inf)
+    _, _, tl, ids = H.token_logprobs(y, allowed[:1].expand(T), n_top=n, temperature=1.5)
+    ids = torch.cat([ids, torch.full((T, 4), -1, device=DEV, dtype=ids.dtype)], 1)
+    tl = torch.cat([tl, torch.zeros(T, 4, device=DEV)], 1)
+    for student in (y, x):
+        loss = H.topk_distill(student, ids, tl, temperature=1.5, tail=True)
+        want, sizes = loss64(student.to(F64) / 1.5, ids, tl)
+        tol = (2 * ulps(V, 12.0) + 2.0 ** -23) * (sizes + 1.0) * 2.25
+        assert bool(torch.isfinite(loss).all()) and bool(((loss.to(F64) - want * 2.25).abs() <= tol).all())
+    assert float(H.topk_distill(y, ids, tl, temperature=1.5, tail=True).abs().max()) <= bound(n + 4) * 2.25
+
+
+@pytest.mark.parametrize("T", [6, 1100])
+def test_mass_that_is_there_stays_infinite_out_of_reach_and_counts_within(H, T):
+    g = gen(T, 6)
+    V = 12
+    y = torch.randn(T, V, device=DEV, generator=g)
+    _, _, tl, ids = H.token_logprobs(y, torch.zeros(T, dtype=torch.long, device=DEV), n_top=V)
+    # a thousandth, and twice the bound: the teacher does leave mass to columns that there are not
+    for left in (1e-3, 2 * bound(V)):
+        assert bool((H.topk_distill(y, ids, tl + math.log1p(-left), tail=True) == math.inf).all())
+    # half the bound counts where a column is free to have it
+    wide = torch.cat([y, torch.full((T, 1), -20.0, device=DEV)], 1)
+    short = tl + math.log1p(-bound(V) / 2)
+    check(H, wide, ids, short, 1.0, g)
