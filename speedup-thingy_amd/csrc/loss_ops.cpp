@@ -77,6 +77,13 @@ Tensor once(Tensor dx, const char* op) {
 
 void* stream_of(AutogradContext* ctx) { return reinterpret_cast<void*>(ctx->saved_data["stream"].toInt()); }
 
+bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// A call that passes its autograd node by would lose a tangent without a word, as a derivative of 0.
+void no_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not implemented");
+}
+
 // ---------------------------------------------------------------- log probabilities from logits
 
 struct Logprobs {
@@ -139,10 +146,10 @@ struct TokenLogprobs : Function<TokenLogprobs> {
   }
 };
 
-bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t n_top,
                                                           double temperature, int64_t stream) {
+  no_tangent("token_logprobs", logits);
   if (wants_grad(logits)) {
     const auto r = TokenLogprobs::apply(logits, tokens, n_top, temperature, stream);
     return {r[0], r[1], r[2], r[3]};
@@ -214,6 +221,8 @@ struct TopkDistill : Function<TopkDistill> {
 
 Tensor topk_distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, double temperature, bool tail,
                     int64_t stream) {
+  no_tangent("topk_distill", logits);
+  no_tangent("topk_distill", teacher);
   const Tensor t = teacher.detach();
   if (wants_grad(logits)) return TopkDistill::apply(logits, ids, t, temperature, tail, stream);
   return distill(logits.detach(), ids, t, temperature, tail, false, stream).loss;
