@@ -106,10 +106,13 @@ class ClusterPoolSwiGLU(nn.Module):
     weights over the selected logits.  Dense parameters (wug, wd) stay the source of truth as in
     StaticClusterPoolSwiGLU (rte/layers.py:119-220).
 
-    Given a list as `balance_into`, each forward appends the routing's (balance loss, router z-loss, counts
-    [ffn_clusters]) to it, for a training program to weigh into its loss (the routing itself gives the router no
-    gradient towards pools a token was not sent to).  The entries hold their graph: the program empties the list
-    once it has its loss, before it captures a backward pass of the same parameters in any case."""
+    Given a list as `balance_into`, each forward that records a graph appends the routing's (balance loss, router
+    z-loss, counts [ffn_clusters]) to it, for a training program to weigh into its loss (the routing itself gives the
+    router no gradient towards pools a token was not sent to).  A pass without gradients appends nothing, nor does a
+    pass within a backward, which is a checkpoint's recomputation: its first pass has left the entry already.  (A
+    reentrant checkpoint makes that first pass without gradients and so leaves none: use_reentrant=False.)  The
+    entries hold their graph: the program empties the list once it has its loss, before it captures a backward pass of
+    the same parameters in any case."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
@@ -128,8 +131,10 @@ class ClusterPoolSwiGLU(nn.Module):
             x, self.router.weight, self.wug.weight, self.wd.weight, self.top_k, resid=resid
         )
         self.last_ids, self.last_weights = ids, w
-        if self.balance_into is not None:
-            self.balance_into.append(self.balance(x, ids))
+        if self.balance_into is not None and torch.is_grad_enabled():
+            entry = self.balance(x, ids)  # in a recomputation too, for what the first pass's entry saved
+            if torch._C._current_graph_task_id() == -1:
+                self.balance_into.append(entry)
         return out
 
     def balance(self, x: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None = None):
