@@ -645,9 +645,10 @@ int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V
  * hidden bf16 [T, d], w bf16 [V, d], logits = hidden w^T (fp32 accumulation); _ok: sizes the tile product
  * takes (d a multiple of 64 from 128, operands below 2 GiB).  fwd: logprob, entropy as
  * rte_token_logprobs_fwd (an infinite logit makes its row NaN), stats f32 [T, 2] for the backward.
- * bwd: dhidden bf16 [T, d] and dw [V, d] (f32 or bf16), NULL = not wanted, for g_logprob / g_entropy f32 [T]
- * (NULL = 0).  The logits are computed again, their gradient in bf16 for `width` (a multiple of 64) tokens of
- * the vocabulary at a time: 2 T width bytes of the workspace. */
+ * bwd: dhidden [T, d] and dw [V, d], NULL = not wanted, for g_logprob / g_entropy f32 [T] (NULL = 0); grads_f32:
+ * 1 = dw in f32, 2 = dhidden in f32 (3 = both), bf16 otherwise.  The logits are computed again, their gradient in
+ * bf16 for `width` (a multiple of 64) tokens of the vocabulary at a time: 2 T width bytes of the workspace.
+ * _bwd_workspace_bytes: need_dh 0 = dhidden not wanted, 1 = in bf16, 2 = in f32; need_dw 0 or 1. */
 int rte_lm_head_logprobs_ok(int T, int d, int V);
 size_t rte_lm_head_logprobs_workspace_bytes(int T, int V);
 int rte_lm_head_logprobs_fwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
@@ -656,7 +657,7 @@ int rte_lm_head_logprobs_fwd(const void* hidden, const void* w, int T, int d, in
 size_t rte_lm_head_logprobs_bwd_workspace_bytes(int T, int d, int V, int width, int need_dh, int need_dw);
 int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
                              float temperature, const float* stats, const float* entropy, const float* g_logprob,
-                             const float* g_entropy, int width, void* dhidden, void* dw, int dw_f32, void* workspace,
+                             const float* g_entropy, int width, void* dhidden, void* dw, int grads_f32, void* workspace,
                              size_t workspace_bytes, void* stream);
 
 /* ---- divergence from a teacher's top logits (no counterpart in the reference, whose

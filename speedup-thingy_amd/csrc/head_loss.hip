@@ -127,10 +127,10 @@ struct Ranges {
 
 struct BwdSpace {
   size_t grad, dh, pad, tail, gemm, total;
-  BwdSpace(int T, int d, int V, const Ranges& r, bool h, bool w) {
+  BwdSpace(int T, int d, int V, const Ranges& r, bool h, bool h_f32, bool w) {
     grad = 0;
-    dh = grad + up((size_t)T * r.most() * sizeof(bf16));
-    pad = dh + (h && !r.one() ? up((size_t)T * d * sizeof(float)) : 0);
+    dh = grad + up((size_t)T * r.most() * sizeof(bf16));  // fp32 sums of several ranges on their way to bf16
+    pad = dh + (h && !h_f32 && !r.one() ? up((size_t)T * d * sizeof(float)) : 0);
     const bool ragged = r.rest8 != r.rest;
     tail = pad + (ragged ? up((size_t)r.rest8 * d * sizeof(bf16)) : 0);
     gemm = tail + (ragged && w ? up((size_t)r.rest8 * d * sizeof(float)) : 0);
@@ -186,12 +186,12 @@ int rte_lm_head_logprobs_fwd(const void* hidden, const void* w, int T, int d, in
 
 size_t rte_lm_head_logprobs_bwd_workspace_bytes(int T, int d, int V, int width, int need_dh, int need_dw) {
   if (!rte_lm_head_logprobs_ok(T, d, V) || width < 64 || width % 64 != 0) return 0;
-  return BwdSpace(T, d, V, Ranges(V, width), need_dh, need_dw).total;
+  return BwdSpace(T, d, V, Ranges(V, width), need_dh, need_dh == 2, need_dw).total;
 }
 
 int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, int V, const int64_t* tokens,
                              float temperature, const float* stats, const float* entropy, const float* g_logprob,
-                             const float* g_entropy, int width, void* dhidden, void* dw, int dw_f32, void* ws,
+                             const float* g_entropy, int width, void* dhidden, void* dw, int grads_f32, void* ws,
                              size_t ws_bytes, void* stream) {
   RTE_REQUIRE(rte_lm_head_logprobs_ok(T, d, V), "lm_head_logprobs_bwd: size not taken (T %d, d %d, V %d)", T, d, V);
   RTE_REQUIRE(width >= 64 && width % 64 == 0, "lm_head_logprobs_bwd: width must be a positive multiple of 64");
@@ -199,9 +199,11 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
   RTE_REQUIRE(hidden && w && tokens && stats && entropy, "lm_head_logprobs_bwd: null argument");
   RTE_REQUIRE(aligned(hidden) && aligned(w) && aligned(dhidden) && aligned(dw) && aligned(ws),
               "lm_head_logprobs_bwd: operands must be 16-byte aligned");
+  RTE_REQUIRE(grads_f32 >= 0 && grads_f32 <= 3, "lm_head_logprobs_bwd: grads_f32 must be in [0, 3]");
   if (!dhidden && !dw) return 0;
+  const bool dw_f32 = grads_f32 & 1, dh_f32 = grads_f32 & 2;
   const Ranges r(V, width);
-  const BwdSpace at(T, d, V, r, dhidden != nullptr, dw != nullptr);
+  const BwdSpace at(T, d, V, r, dhidden != nullptr, dh_f32, dw != nullptr);
   RTE_REQUIRE((int64_t)T * r.most() < (int64_t)1 << 30, "lm_head_logprobs_bwd: width too large for %d rows", T);
   RTE_REQUIRE(ws && ws_bytes >= at.total, "lm_head_logprobs_bwd: workspace too small");
   auto s = static_cast<hipStream_t>(stream);
@@ -209,6 +211,8 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
   void* grad = base + at.grad;
   void* gemm_ws = base + at.gemm;
   const size_t gemm_bytes = at.total - at.gemm;
+  // sums of several ranges are kept in fp32
+  const bool dh_sum = !dh_f32 && !r.one();
   float* dh32 = reinterpret_cast<float*>(base + at.dh);
   for (int lo = 0; lo < V;) {
     const bool last = lo == r.whole;  // the columns past the whole 64s
@@ -236,8 +240,8 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
     e.inv_t = 1.0f / temperature;
     e.vocab = V;
     RTE_TRY(tiles(wr, hidden, n, T, d, e, EPI_DLOGITS, s));
-    if (dhidden)  // [T, n] [n, d]; in fp32 until the last of several ranges
-      RTE_TRY(product(grad, n, 0, wr, d, 1, r.one() ? dhidden : dh32, !r.one(), T, d, n, lo > 0 ? 1.0f : 0.0f, gemm_ws,
+    if (dhidden)  // [T, n] [n, d]
+      RTE_TRY(product(grad, n, 0, wr, d, 1, dh_sum ? dh32 : dhidden, dh_f32 || dh_sum, T, d, n, lo > 0 ? 1.0f : 0.0f, gemm_ws,
                       gemm_bytes, s));
     if (dw) {     // [n, T] [T, d]
       void* out = static_cast<char*>(dw) + (int64_t)lo * d * (dw_f32 ? 4 : 2);
@@ -253,7 +257,7 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
     }
     lo += real;
   }
-  return dhidden && !r.one() ? cast_f32_bf16(dh32, (int64_t)T * d, static_cast<bf16*>(dhidden), s) : 0;
+  return dhidden && dh_sum ? cast_f32_bf16(dh32, (int64_t)T * d, static_cast<bf16*>(dhidden), s) : 0;
 }
 
 }  // extern "C"

@@ -327,21 +327,21 @@ struct HeadLogprobs : Function<HeadLogprobs> {
     const Tensor gl = row_grad(g[0]), ge = row_grad(g[1]);
     const int64_t T = hb.size(0), d = hb.size(1), V = wb.size(0);
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
-    const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
-    const bool w_bf16 = w_dtype == at::kBFloat16;
+    const auto h_dtype = ctx->saved_data["h_dtype"].toScalarType(), w_dtype = ctx->saved_data["w_dtype"].toScalarType();
+    const bool h_bf16 = h_dtype == at::kBFloat16, w_bf16 = w_dtype == at::kBFloat16;
     int64_t width = ctx->saved_data["grad_bytes"].toInt() / (2 * T);
     width = std::max<int64_t>(64, std::min(width, V) / 64 * 64);
     Tensor dh, dw;
-    if (need_h) dh = at::empty({T, d}, hb.options());
+    if (need_h) dh = at::empty({T, d}, hb.options().dtype(h_bf16 ? at::kBFloat16 : at::kFloat));
     if (need_w) dw = at::empty({V, d}, hb.options().dtype(w_bf16 ? at::kBFloat16 : at::kFloat));
-    const size_t n = rte_lm_head_logprobs_bwd_workspace_bytes((int)T, (int)d, (int)V, (int)width, need_h, need_w);
+    const int dh_type = need_h ? (h_bf16 ? 1 : 2) : 0;
+    const size_t n = rte_lm_head_logprobs_bwd_workspace_bytes((int)T, (int)d, (int)V, (int)width, dh_type, need_w);
     const Tensor ws = scratch(n, hb);
     ok(rte_lm_head_logprobs_bwd(hb.data_ptr(), wb.data_ptr(), (int)T, (int)d, (int)V, ptr<int64_t>(saved[2]),
                                 (float)ctx->saved_data["temperature"].toDouble(), ptr<float>(saved[3]), ptr<float>(saved[4]),
-                                ptr<float>(gl), ptr<float>(ge), (int)width, ptr<void>(dh), ptr<void>(dw), !w_bf16,
-                                ptr<void>(ws), n, stream_of(ctx)),
+                                ptr<float>(gl), ptr<float>(ge), (int)width, ptr<void>(dh), ptr<void>(dw),
+                                (w_bf16 ? 0 : 1) + (h_bf16 ? 0 : 2), ptr<void>(ws), n, stream_of(ctx)),
        "rte_lm_head_logprobs_bwd");
-    const auto h_dtype = ctx->saved_data["h_dtype"].toScalarType();
     if (need_h) out[0] = once(dh.view(ctx->saved_data["shape"].toIntVector()).to(h_dtype), "lm_head_logprobs");
     if (need_w) out[1] = once(dw.to(w_dtype), "lm_head_logprobs");
     return out;
