@@ -1681,8 +1681,8 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         T, V = hb.shape[0], wb.shape[0]
         need_h, need_w = ctx.needs_input_grad[:2]
         gl, ge = (None if g is None else _dense(g, F32).view(T) for g in (g_lp, g_ent))
-        dh = torch.empty(hb.shape, dtype=BF16 if h_dt == BF16 else F32, device=hb.device)
-        dw = torch.zeros(wb.shape, dtype=F32, device=hb.device)
+        dh = torch.empty(hb.shape, dtype=BF16 if h_dt == BF16 else F32, device=hb.device) if need_h else None
+        dw = torch.zeros(wb.shape, dtype=F32, device=hb.device) if need_w else None
         wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
         for lo in range(0, T, LMHeadLogprobsFn.ROWS):
             hi = min(T, lo + LMHeadLogprobsFn.ROWS)
