@@ -1682,22 +1682,24 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         need_h, need_w = ctx.needs_input_grad[:2]
         gl, ge = (None if g is None else _dense(g, F32).view(T) for g in (g_lp, g_ent))
         dh = torch.empty(hb.shape, dtype=BF16 if h_dt == BF16 else F32, device=hb.device) if need_h else None
-        dw = torch.zeros(wb.shape, dtype=F32, device=hb.device) if need_w else None
         wp = wb if V % 8 == 0 else torch.nn.functional.pad(wb, (0, 0, 0, -V % 8))
+        dw = (torch.empty if T else torch.zeros)(wp.shape, dtype=F32, device=hb.device) if need_w else None
         for lo in range(0, T, LMHeadLogprobsFn.ROWS):
             hi = min(T, lo + LMHeadLogprobsFn.ROWS)
             logits = gemm(hb[lo:hi], wb, out_f32=True, own_ws=True)
             dl = torch.empty_like(logits)
             call("rte_token_logprobs_bwd", ptr(logits), V, 1, hi - lo, V, ptr(tk[lo:]), temperature, ptr(stats[lo:]),
                  ptr(ent[lo:]), None if gl is None else ptr(gl[lo:]), None if ge is None else ptr(ge[lo:]), ptr(dl), _s())
-            dl = dl.to(BF16)
+            dl = cast_bf16(dl)
             if V % 8:
                 dl = torch.nn.functional.pad(dl, (0, -V % 8))
             if need_h:
                 gemm(dl, wp, b_t=True, out=dh[lo:hi], own_ws=True)
             if need_w:
-                dw += gemm(dl, hb[lo:hi], a_t=True, b_t=True, out_f32=True, own_ws=True)[:V]
-        return dh.view(shape).to(h_dt) if need_h else None, dw.to(w_dt) if need_w else None, None, None, None, None
+                gemm(dl, hb[lo:hi], a_t=True, b_t=True, out=dw, beta=float(lo > 0), own_ws=True)
+        if need_w:
+            dw = cast_bf16(dw[:V]) if w_dt == BF16 else dw[:V].to(w_dt)
+        return dh.view(shape).to(h_dt) if need_h else None, dw, None, None, None, None
 
 
 def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:

@@ -98,3 +98,23 @@ def test_nothing_is_allocated_for_a_gradient_that_is_not_wanted(H, want):
     logits = min(T, 2048) * V * 4
     assert (h if want == "hidden" else w).grad is not None
     assert peak < 3 * logits + (1 << 23 if want == "weights" else 1 << 24), peak
+
+
+def test_backward_of_narrow_widths_runs_on_the_framework_s_kernels(H):
+    """Sums over blocks of rows and roundings to bf16 are the products' and the cast's own; torch converts and adds
+    nothing."""
+    from torch.profiler import ProfilerActivity, profile
+
+    g = gen(4)
+    T, d, V = 4500, 64, 136
+    h = torch.randn(T, d, device=DEV, generator=g).bfloat16().requires_grad_()
+    w = (torch.randn(V, d, device=DEV, generator=g) * 0.2).bfloat16().requires_grad_()
+    tok = torch.randint(0, V, (T,), device=DEV, generator=g)
+    up = torch.randn(T, device=DEV, generator=g)
+    lp, _ = H.lm_head_logprobs(h, w, tok)
+    with profile(activities=[ProfilerActivity.CPU]) as prof:
+        torch.autograd.grad(lp, (h, w), up)
+    torch.cuda.synchronize()
+    names = {e.key for e in prof.key_averages()}
+    assert "aten::empty" in names  # the backward's thread is seen
+    assert not names & {"aten::_to_copy", "aten::copy_", "aten::add_", "aten::add"}, names
