@@ -10,11 +10,13 @@ from __future__ import annotations
 import ctypes
 import os
 from pathlib import Path
+from types import SimpleNamespace
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "librte_hip.so"
 OPS_PATH = LIB_PATH.with_name("librte_ops.so")  # autograd nodes in C++ over librte_hip (torch.ops.rte)
+OPS = ("token_logprobs", "topk_distill", "pool_balance", "lm_head_logprobs")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -226,15 +228,17 @@ _OPS = None
 
 
 def ops():
-    """torch.ops.rte: the token losses and the pool balance with their gradients (csrc/loss_ops.cpp); raises if
-    the library is not built."""
+    """The token losses and the pool balance with their gradients (csrc/loss_ops.cpp, torch.ops.rte); raises if the
+    library is not built.  The operators' own functions, past torch.ops: a program under torch.compile runs them between
+    its graphs, as the framework's other operators, where torch.ops' handles would be traced into a graph with operands
+    that have no memory."""
     global _OPS
     if _OPS is None:
         load()
         if not OPS_PATH.exists():
             raise RuntimeError(f"{OPS_PATH} is not built; run speedup-thingy_amd/build.py")
         torch.ops.load_library(str(OPS_PATH))
-        _OPS = torch.ops.rte
+        _OPS = SimpleNamespace(**{name: torch._C._jit_get_operation(f"rte::{name}")[0] for name in OPS})
     return _OPS
 
 
