@@ -851,6 +851,7 @@ __global__ void __launch_bounds__(256)
   const float g = g_lp && tok >= 0 && tok < V ? g_lp[t] : 0.0f, gh = g_ent ? g_ent[t] : 0.0f;
   const float gc = g + gh * entropy[t];
   const bool empty = log_s == -INFINITY;
+  const bool none = empty || (gh == 0.0f && (tok < 0 || tok >= V));  // padding's logits may hold anything
   // the token's column is written again by the lane that holds it
   const int64_t rel = tok - c0;
   const bool mine = g != 0.0f && !empty && rel >= 0 && rel < len && (int)(rel / VE) % 64 == lane;
@@ -864,7 +865,7 @@ __global__ void __launch_bounds__(256)
     if ((i * 64) * VE >= len) continue;
     float d[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) d[j] = empty ? 0.0f : slope(Row<X>::get(w[i], j));
+    for (int j = 0; j < VE; ++j) d[j] = none ? 0.0f : slope(Row<X>::get(w[i], j));
     store_words(out, (i * 64 + lane) * VE, len, d);
   }
   if (mine) Row<X>::put(out, rel, slope(at_tok) + g * inv_t);
