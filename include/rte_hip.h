@@ -644,7 +644,8 @@ int rte_token_logprobs_bwd(const void* logits, int64_t ld, int f32, int T, int V
  *      in the reference; beside rte_gemm_bf16 + rte_ce_fwd) ----
  * hidden bf16 [T, d], w bf16 [V, d], logits = hidden w^T (fp32 accumulation); _ok: sizes the tile product
  * takes (d a multiple of 64 from 128, operands below 2 GiB).  fwd: logprob, entropy as
- * rte_token_logprobs_fwd (an infinite logit makes its row NaN), stats f32 [T, 2] for the backward.
+ * rte_token_logprobs_fwd (an infinite logit makes its row NaN), stats f32 [T, 2] for the backward; the workspace
+ * holds 16 bytes per row for every 64 columns.
  * bwd: dhidden [T, d] and dw [V, d], NULL = not wanted, for g_logprob / g_entropy f32 [T] (NULL = 0); grads_f32:
  * 1 = dw in f32, 2 = dhidden in f32 (3 = both), bf16 otherwise.  The logits are computed again, their gradient in
  * bf16 for `width` (a multiple of 64) tokens of the vocabulary at a time: 2 T width bytes of the workspace.

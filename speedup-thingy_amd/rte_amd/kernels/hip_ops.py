@@ -1625,7 +1625,9 @@ def token_logprobs(logits, tokens, *, n_top: int = 0, temperature: float = 1.0):
     the vocabulary NaN.  entropy [...] float32: -sum p log p.  top_logprobs float32 / top_ids int32 [..., n_top]:
     the n_top <= 128 largest logits, value descending, ties to the lower id, NaN first.  logprob and entropy are
     differentiable; the alternatives carry no gradient (they make topk_distill's targets).  A row with no logit
-    above -inf has log probabilities -inf, entropy 0 and gradient 0; a NaN or +inf logit makes its row NaN."""
+    above -inf has log probabilities -inf, entropy 0 and gradient 0; a NaN or +inf logit makes its row NaN.  The last
+    bits of a row may differ in a call of another size (this and the other losses of rows here), never with what the
+    other rows hold."""
     _lib.require_device_tensors("token_logprobs", logits, tokens)
     _same_device("token_logprobs", logits, tokens)
     _check_logits("token_logprobs", logits)
@@ -1703,9 +1705,15 @@ class LMHeadLogprobsFn(torch.autograd.Function):
 
 
 def lm_head_logprobs(hidden, w, tokens, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
-    """(logprob, entropy) of token_logprobs for the logits hidden [..., d] @ w [V, d]^T, which are never stored
-    whole: memory grows with the tokens, not with tokens times vocabulary.  bf16 operands and fp32 logits as
-    in lm_head_ce; both results are differentiable in hidden and w."""
+    """(logprob, entropy) of token_logprobs for the logits hidden [..., d] @ w [V, d]^T, without the logits: the forward
+    keeps 16 bytes per token for every 64 columns while it runs (a 16th of fp32 logits), the backward bf16 gradients of the
+    logits, 1 GiB of them at a time.  Widths under 128 or not a multiple of 64 and operands of 2 GiB and more go by fp32
+    logits of 2048 tokens at a time, the fp32 precision stores them all.
+
+    bf16 operands and fp32 logits as in lm_head_ce; both results are differentiable in hidden and w.  The logits'
+    gradient is rounded to bf16 before the products that sum it, and what they sum to is the gradient in fp32, or rounded
+    once more for bf16 operands.  Padding (negative tokens) needs finite hidden states: the weights' gradient multiplies
+    them by 0."""
     _lib.require_device_tensors("lm_head_logprobs", hidden, w, tokens)
     _same_device("lm_head_logprobs", hidden, w, tokens)
     _whole_numbers("lm_head_logprobs", tokens)
