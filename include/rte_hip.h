@@ -671,6 +671,8 @@ int rte_lm_head_logprobs_bwd(const void* hidden, const void* w, int T, int d, in
  *           loss = temperature^2 (sum_j p_j (log p_j - log q_j) + r (log r - log q(not listed)))
  *           where the row holds no unlisted logit above -inf, an r of at most 2^-23 (K + 32), the rounding of
  *           K log probabilities, is 0; with a larger one the loss is infinite
+ *   tail 2, 3: as 1, of values that were rounded to bf16 (2) or fp16 (3) before: there r may be larger by
+ *           17/16 of half a step, 2^-8 or 2^-11, times sum_j p_j |teacher_j|
  * A row without entries (tail 0: or without one above -inf) has loss 0 and no gradient; an id past the
  * vocabulary makes the loss NaN and the gradient 0.  K <= 128.
  * Kept for the backward (stats NULL: nothing is): stats f32 [T, 2], cols int32 [T, K] = the columns that count

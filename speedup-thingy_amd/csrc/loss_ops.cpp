@@ -182,10 +182,12 @@ Distill distill(const Tensor& logits, const Tensor& ids, const Tensor& teacher, 
     r.cols = at::empty({T, K}, f32.dtype(at::kInt));
     r.coef = at::empty({T, K}, f32);
   }
+  const auto kept = teacher.scalar_type();
+  const int rest = !tail ? 0 : kept == at::kBFloat16 ? 2 : kept == at::kHalf ? 3 : 1;
   const size_t n = rte_topk_distill_workspace_bytes((int)T, (int)V, (int)K);
   const Tensor ws = scratch(n, r.loss);
   ok(rte_topk_distill_fwd(r.rows.data_ptr(), r.ld, logits.scalar_type() == at::kFloat, (int)T, (int)V, ptr<int32_t>(ic),
-                          ptr<float>(tc), (int)K, (float)temperature, tail, ptr<float>(r.loss), ptr<float>(r.stats),
+                          ptr<float>(tc), (int)K, (float)temperature, rest, ptr<float>(r.loss), ptr<float>(r.stats),
                           ptr<int32_t>(r.cols), ptr<float>(r.coef), ptr<void>(ws), n, reinterpret_cast<void*>(stream)),
      "rte_topk_distill_fwd");
   return r;

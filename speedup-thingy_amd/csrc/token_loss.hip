@@ -73,6 +73,7 @@ struct RowArgs {
   const float* tl;
   int K, tail;
   double it, t2;
+  double kept;  // half a step, and a sixteenth of it, of the type that the teacher's values were kept in (0: fp32)
   float* loss;
   int32_t* cols;
   float* coef;
@@ -194,7 +195,12 @@ __device__ void finish_distill(const RowArgs& a, const X* row, int64_t t, const 
   // What roundings leave of 1 is no mass outside the list, which would make the loss infinite where the student can have
   // none there.  fp32 log probabilities of a row with K possible columns leave at most 2^-24 (K + 2 + 7 log K): K + 2 from
   // the exponentials and their sum, the rest from exponents, logarithm and results, each weighted by p; log K < 5.
-  if (rest.s == 0.0f && r <= (a.K + 32) * 0x1p-23) r = 0.0;
+  // Values kept in 16 bits are off by half a step of each, e^x - 1 < 17/16 x: so much of p_j |t_j| more.
+  if (rest.s == 0.0f && r > 0.0) {
+    double most = (a.K + 32) * 0x1p-23;
+    if (a.kept != 0.0) most += a.kept * wave_sum((p[0] > 0.0 ? p[0] * -lp[0] : 0.0) + (p[1] > 0.0 ? p[1] * -lp[1] : 0.0));
+    if (r <= most) r = 0.0;
+  }
   // the rest's own sum: times its scale it may be below the least number, however finite its logarithm
   const double logs = log(lane == 0 ? total : lane == 1 ? tsum : lane == 2 ? r : (double)rest.s);
   const double inverses = 1.0 / (lane == 0 ? total : tsum);
@@ -1026,6 +1032,7 @@ int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, 
                          int32_t* cols, float* coef, void* ws, size_t ws_bytes, void* stream) {
   RTE_REQUIRE(T >= 0 && V >= 1 && ld >= 0, "topk_distill: bad sizes");
   RTE_REQUIRE(K >= 1 && K <= kMaxTop, "topk_distill: list length must be in [1, %d]", kMaxTop);
+  RTE_REQUIRE(tail >= 0 && tail <= 3, "topk_distill: tail must be in [0, 3]");
   RTE_REQUIRE(temperature > 0.0f && temperature < INFINITY, "topk_distill: temperature must be positive and finite");
   if (T == 0) return 0;
   RTE_REQUIRE(logits && ids && teacher && loss && (!stats || (cols && coef)), "topk_distill: null argument");
@@ -1036,6 +1043,7 @@ int rte_topk_distill_fwd(const void* logits, int64_t ld, int f32, int T, int V, 
   a.ld = ld, a.T = T, a.V = V;
   a.inv_t = 1.0f / temperature, a.c2 = (float)(1.4426950408889634 / temperature);
   a.ids = ids, a.tl = teacher, a.K = K, a.tail = tail, a.it = 1.0 / temperature;
+  a.kept = tail == 2 ? 0x1.1p-8 : tail == 3 ? 0x1.1p-11 : 0.0;
   a.t2 = (double)temperature * temperature, a.loss = loss, a.stats = stats, a.cols = cols, a.coef = coef;
   auto s = static_cast<hipStream_t>(stream);
   return f32 ? launch_rows<float, true, false>(logits, a, ws, s) : launch_rows<bf16, true, false>(logits, a, ws, s);

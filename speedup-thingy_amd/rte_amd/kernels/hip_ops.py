@@ -1747,8 +1747,8 @@ def topk_distill(logits, teacher_ids, teacher_logits, *, temperature: float = 1.
     do as well).  tail True: teacher_logits are log probabilities at this temperature (token_logprobs(...,
     temperature=...)), and what they leave of 1 is compared with the student's mass outside the list, so the
     loss is 0 where both agree on the list and on the rest.  Where the student can reach no column outside the list, a
-    remainder within the rounding of K fp32 log probabilities, 2^-23 (K + 32), is none; a larger one makes the loss
-    infinite.
+    remainder within the rounding of K fp32 log probabilities, 2^-23 (K + 32), is none, nor is one within the half steps of
+    values kept in bfloat16 or float16; a larger one makes the loss infinite.
 
     Negative ids are no entries; of a repeated id the first counts.  A row without entries (tail False: without one above -inf)
     has loss 0 and no gradient; an id past the vocabulary makes the row's loss NaN and its gradient 0."""
